@@ -38,9 +38,11 @@ extern "C" {
 
 /* Element types (values of XLA_FFI_DataType). */
 #define T0B_S32 4
+#define T0B_F16 10   /* routed operators only */
 #define T0B_F32 11
 #define T0B_F64 12
 #define T0B_C64 15
+#define T0B_BF16 16  /* routed operators only */
 #define T0B_C128 18
 
 /* Plan operations (the reference's operation codes, descriptor.h:69-78). */
@@ -274,6 +276,100 @@ int t0b_sector_gemm(int32_t dtype, int64_t sectors, const int64_t* host_table,
                     const int64_t* device_table, const void* left, int64_t left_size,
                     const void* right, int64_t right_size, void* output, int64_t output_size,
                     void* stream, char* error, size_t error_size);
+
+/*
+ * Routed operators: block-sparse products whose sectors ("experts") are chosen
+ * per token at run time, on the device, with their gradients.  An entry is one
+ * (token, slot) pair, number token * top_k + slot; expert-ordered row p holds
+ * entry rows[p], and expert e's rows are [offsets[e], offsets[e + 1]).  Entries
+ * without an expert are ordered last, from offsets[experts] on.  Row strides are
+ * in elements.  rows, positions and offsets are the device arrays t0b_route
+ * writes; kernels skip an address outside the stated operand.  Outputs are
+ * contiguous and must not overlap inputs.
+ *
+ * t0b_route: scores s = softmax (score 0) or sigmoid (score 1) of the token's
+ * logits (F32, F16, BF16); choice c = s + bias, or the logits where bias is
+ * NULL and group_best is 1; the top_groups of `groups` equal expert groups by
+ * their best c (group_best 1) or the sum of their two best (2); then the top_k
+ * best c, ties to the lowest index.  weights = scale * s, divided by the sum of
+ * the chosen s + 1e-20 if renormalize is 1.  A logit of -inf or NaN takes no
+ * expert; a token with mask 0 takes none and its logits are not read.  Missing
+ * choices have index -1, weight 0 and position -1.  experts <= 512, top_k <= 32,
+ * groups <= 32, tokens * top_k < 2^31.  workspace: t0b_route_workspace() bytes,
+ * 4-byte aligned (may be NULL when that is 0).
+ */
+size_t t0b_route_workspace(int64_t tokens, int32_t experts);
+int t0b_route(int32_t dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups,
+              int32_t group_best, int32_t score, int32_t renormalize, float scale, const void* logits,
+              int64_t logit_stride, const float* bias, const uint8_t* mask, int32_t* chosen, float* weights,
+              int32_t* rows, int32_t* positions, int32_t* offsets, void* workspace, size_t workspace_size,
+              void* stream, char* error, size_t error_size);
+
+/* Gradient of t0b_route's weights with respect to the logits (the choice is
+ * piecewise constant; the bias only enters the choice).  logits_grad [tokens,
+ * experts] of the logits' dtype; zero for tokens without an expert. */
+int t0b_route_backward(int32_t dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t score,
+                       int32_t renormalize, float scale, const void* logits, int64_t logit_stride,
+                       const int32_t* chosen, const float* weights_grad, void* logits_grad, void* stream,
+                       char* error, size_t error_size);
+
+/*
+ * output[p] = x[r(p)] @ w[e] (transposed 0) or x[r(p)] @ w[e]^T (1) for every
+ * row p of every expert e; w [experts, inner, outer]; r(p) = rows[p] / top_k
+ * with gather 1, else p; x has x_rows rows.  output [entries, outer or inner];
+ * rows without an expert are zero.  F16 or BF16, summed in 32 bits, rounded once.
+ */
+int t0b_routed_product(int32_t dtype, int32_t transposed, int64_t entries, int32_t experts, int32_t top_k,
+                       int32_t inner, int32_t outer, int32_t gather, const void* x, int64_t x_rows, int64_t x_stride,
+                       const void* w, const int32_t* rows, const int32_t* offsets, void* output, void* stream,
+                       char* error, size_t error_size);
+
+/* output[e] = sum over e's rows p of x[r(p)]^T y[q(p)], [experts, inner, outer];
+ * zero for an expert without rows.  gather_x / gather_y as above for r and q. */
+int t0b_routed_weight_grad(int32_t dtype, int64_t entries, int32_t experts, int32_t top_k, int32_t inner,
+                           int32_t outer, int32_t gather_x, const void* x, int64_t x_rows, int64_t x_stride,
+                           int32_t gather_y, const void* y, int64_t y_rows, int64_t y_stride, const int32_t* rows,
+                           const int32_t* offsets, void* output, void* stream, char* error, size_t error_size);
+
+/* output[t] = sum over slots of y[positions[t, slot]] (absent slots skipped),
+ * y [tokens * top_k, width] with row stride y_stride, output [tokens, width]. */
+int t0b_routed_sum(int32_t dtype, int64_t tokens, int32_t top_k, int32_t width, const void* y, int64_t y_stride,
+                   const int32_t* positions, void* output, void* stream, char* error, size_t error_size);
+
+/*
+ * Gated activation a = w * silu(g) * u of rows h = [g | u] (width each), with h
+ * kept in 8 bits: codes [rows, 2 * width], scales [rows, 2 * ceil(width / group)],
+ * group 32, 64 or 128 neighbours of one half (scale = max|h| / 127, codes rounded
+ * half to even; a group with a NaN or infinity loads as NaN; one below 2^-100 as
+ * zeros).  w = weights[rows[p]] with a routing, else 1 (weights, row_entries and
+ * offsets all NULL); rows without an expert are not read and give zeros.
+ */
+int t0b_gated_save(int32_t dtype, int64_t row_count, int32_t width, int32_t group, const void* h, int64_t h_stride,
+                   const float* weights, const int32_t* row_entries, const int32_t* offsets, int32_t experts,
+                   void* a, int8_t* codes, float* scales, void* stream, char* error, size_t error_size);
+
+/* The gradient from the checkpoint: h_grad [rows, 2 * width], the activation
+ * again (a, for the next product's weight gradient) and the routing weights'
+ * gradient [rows] in entry order (may be NULL). */
+int t0b_gated_backward(int32_t dtype, int64_t row_count, int32_t width, int32_t group, const int8_t* codes,
+                       const float* scales, const void* a_grad, int64_t a_grad_stride, const float* weights,
+                       const int32_t* row_entries, const int32_t* offsets, int32_t experts, void* h_grad, void* a,
+                       float* weights_grad, void* stream, char* error, size_t error_size);
+
+/* values[i] = codes[i] * its group's scale, as F32, F16 or BF16. */
+int t0b_checkpoint_load(int32_t dtype, int64_t row_count, int32_t width, int32_t group, const int8_t* codes,
+                        const float* scales, void* values, void* stream, char* error, size_t error_size);
+
+/*
+ * output[p][n] = sum over k of scale[e][n][k / group] * (q[e][n][k] - 8) * x[r(p)][k]
+ * for few rows (single tokens): codes [experts, outer, inner / 2] hold two 4-bit
+ * weights per byte, the even k in the low half, 16-byte aligned; scales [experts,
+ * outer, inner / group] of x's dtype; group 32, 64 or 128 divides inner.
+ */
+int t0b_routed_matvec4(int32_t dtype, int64_t entries, int32_t experts, int32_t top_k, int32_t inner, int32_t outer,
+                       int32_t group, int32_t gather, const void* x, int64_t x_rows, int64_t x_stride,
+                       const uint8_t* codes, const void* scales, const int32_t* rows, const int32_t* offsets,
+                       void* output, void* stream, char* error, size_t error_size);
 
 /* Number of kernels this library launched since load (for launch accounting). */
 uint64_t t0b_kernel_launches(void);

@@ -13,7 +13,7 @@ from . import build as _build
 
 LIBRARY_PATH = _build.LIBRARY
 
-S32, F32, F64, C64, C128 = 4, 11, 12, 15, 18
+S32, F16, F32, F64, C64, BF16, C128 = 4, 10, 11, 12, 15, 16, 18
 OP_COPY, OP_UPDATE, OP_DOT, OP_ACCUMULATION, OP_REDUCTION, OP_GROUPED = 0, 1, 2, 3, 4, 5
 PLAN_OUTPUTS_DISJOINT = 1
 PLAN_WIDE_OFFSETS = 2
@@ -78,6 +78,33 @@ SIGNATURES = {
     "t0b_sector_gemm": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, c_i64p, ctypes.c_void_p, ctypes.c_void_p,
                                        ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                        ctypes.c_int64, ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_route_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32]),
+    "t0b_route": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, *[ctypes.c_int32] * 7, ctypes.c_float,
+                                 ctypes.c_void_p, ctypes.c_int64, *[ctypes.c_void_p] * 8, ctypes.c_size_t,
+                                 ctypes.c_void_p, ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_route_backward": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, *[ctypes.c_int32] * 4, ctypes.c_float,
+                                          ctypes.c_void_p, ctypes.c_int64, *[ctypes.c_void_p] * 4, ctypes.c_char_p,
+                                          ctypes.c_size_t]),
+    "t0b_routed_product": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, *[ctypes.c_int32] * 5,
+                                          ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, *[ctypes.c_void_p] * 5,
+                                          ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_routed_weight_grad": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, *[ctypes.c_int32] * 5, ctypes.c_void_p,
+                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p,
+                                              ctypes.c_int64, ctypes.c_int64, *[ctypes.c_void_p] * 4,
+                                              ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_routed_sum": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                      ctypes.c_int64, *[ctypes.c_void_p] * 3, ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_gated_save": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                      ctypes.c_int64, *[ctypes.c_void_p] * 3, ctypes.c_int32,
+                                      *[ctypes.c_void_p] * 4, ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_gated_backward": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                          *[ctypes.c_void_p] * 3, ctypes.c_int64, *[ctypes.c_void_p] * 3,
+                                          ctypes.c_int32, *[ctypes.c_void_p] * 4, ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_checkpoint_load": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                           *[ctypes.c_void_p] * 4, ctypes.c_char_p, ctypes.c_size_t]),
+    "t0b_routed_matvec4": (ctypes.c_int, [ctypes.c_int32, ctypes.c_int64, *[ctypes.c_int32] * 6, ctypes.c_void_p,
+                                          ctypes.c_int64, ctypes.c_int64, *[ctypes.c_void_p] * 6, ctypes.c_char_p,
+                                          ctypes.c_size_t]),
     "t0b_kernel_launches": (ctypes.c_uint64, []),
 }
 

@@ -5,14 +5,13 @@
 
 #include "engine.h"
 #include "gemm.h"
+#include "guard.h"
 #include "layout.h"
 #include "plan.h"
 
 #include <atomic>
-#include <cstdio>
 #include <cstring>
 #include <memory>
-#include <new>
 
 struct t0b_plan {
   t0b::Plan plan;
@@ -22,33 +21,12 @@ struct t0b_plan {
 
 namespace {
 
+using t0b::Bytes;
+using t0b::Disjoint;
+using t0b::Guard;
+
 std::atomic<uint64_t> g_created{0};
 std::atomic<uint64_t> g_destroyed{0};
-
-void Message(char* error, size_t size, const char* text) {
-  if (error != nullptr && size != 0) std::snprintf(error, size, "%s", text);
-}
-
-// Run `body`, mapping invalid arguments to 1 and everything else to 2.
-template <typename Body>
-int Guard(char* error, size_t size, Body&& body) {
-  try {
-    body();
-    return 0;
-  } catch (const t0b::InvalidArgument& e) {
-    Message(error, size, (std::string("tensor0-b200: ") + e.what()).c_str());
-    return 1;
-  } catch (const std::bad_alloc&) {
-    Message(error, size, "tensor0-b200: out of host memory");
-    return 2;
-  } catch (const std::exception& e) {
-    Message(error, size, (std::string("tensor0-b200: ") + e.what()).c_str());
-    return 2;
-  } catch (...) {
-    Message(error, size, "tensor0-b200: unknown exception");
-    return 2;
-  }
-}
 
 int ElementBytes(int32_t dtype) {
   switch (dtype) {
@@ -66,22 +44,6 @@ int CoefficientBytes(int32_t coefficient, int32_t storage) {
   if (coefficient == (single ? T0B_F32 : T0B_F64)) return single ? 4 : 8;
   if (complex && coefficient == (single ? T0B_C64 : T0B_C128)) return single ? 8 : 16;
   throw t0b::InvalidArgument("unsupported CUDA coefficient dtype; expected S32 or matching real/complex precision");
-}
-
-uint64_t Bytes(uint64_t elements, uint64_t item) {
-  uint64_t out = 0;
-  if (!t0b::CheckedMul(elements, item, &out) || out > static_cast<uint64_t>(PTRDIFF_MAX)) {
-    throw t0b::InvalidArgument("buffer size exceeds addressable storage");
-  }
-  return out;
-}
-
-// The reference's overlap rule (ffi/buffers.h:43-52).
-void Disjoint(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
-  if (a_bytes == 0 || b_bytes == 0) return;
-  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  const bool overlap = x <= y ? y - x < a_bytes : x - y < b_bytes;
-  if (overlap) throw t0b::InvalidArgument("input and output buffers overlap");
 }
 
 // Storage buffers are aligned to their element size: the map engine copies

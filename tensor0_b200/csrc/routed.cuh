@@ -1,0 +1,99 @@
+// Device helpers shared by the routed operators.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace t0b {
+
+// XLA_FFI_DataType codes of the types these operators take.
+constexpr int32_t kTypeF16 = 10, kTypeF32 = 11, kTypeBf16 = 16;
+
+__device__ __forceinline__ float ToFloat(float v) { return v; }
+__device__ __forceinline__ float ToFloat(__half v) { return __half2float(v); }
+__device__ __forceinline__ float ToFloat(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T> __device__ __forceinline__ T FromFloat(float v);
+template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half FromFloat<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 FromFloat<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Two floats rounded into one 32-bit word (the first in the low half).
+template <typename T> __device__ __forceinline__ uint32_t Pack2(float a, float b) {
+  const T lo = FromFloat<T>(a), hi = FromFloat<T>(b);
+  return static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&lo)) |
+         (static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&hi)) << 16);
+}
+template <> __device__ __forceinline__ uint32_t Pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t Pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T> __device__ __forceinline__ float2 Unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 Unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <> __device__ __forceinline__ float2 Unpack2<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// Eight neighbouring values of a row as floats.  Vector: one 16-byte access
+// (p is 16-byte aligned and all eight lie in the row); otherwise value by
+// value, `count` of them (the others read as 0 and are not written).
+template <typename T, bool Vector>
+__device__ __forceinline__ void Load8(const T* p, int count, float (&v)[8]) {
+  if constexpr (Vector) {
+    if (count <= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      return;
+    }
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Unpack2<T>(w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < count ? ToFloat(p[i]) : 0.0f;
+  }
+}
+
+template <typename T, bool Vector>
+__device__ __forceinline__ void Store8(T* p, int count, const float (&v)[8]) {
+  if constexpr (Vector) {
+    if (count <= 0) return;
+    *reinterpret_cast<uint4*>(p) = make_uint4(Pack2<T>(v[0], v[1]), Pack2<T>(v[2], v[3]), Pack2<T>(v[4], v[5]),
+                                              Pack2<T>(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i < count) p[i] = FromFloat<T>(v[i]);
+    }
+  }
+}
+
+// An expert's first row as read from the device, kept inside the rows there are.
+__device__ __forceinline__ int64_t RowBound(int32_t offset, int64_t entries) {
+  return offset < 0 ? 0 : offset < entries ? offset : entries;
+}
+
+// Streaming multiprocessors of the current device.
+inline int RoutedSmCount() {
+  int device = 0, count = 148;
+  if (cudaGetDevice(&device) == cudaSuccess) {
+    cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+  }
+  return count;
+}
+
+}  // namespace t0b
