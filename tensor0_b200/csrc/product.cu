@@ -151,9 +151,10 @@ void Sum(const RoutedSumArgs& a, cudaStream_t stream) {
 }  // namespace
 
 void LaunchProduct(int kind, int32_t dtype, const ProductArgs& args, cudaStream_t stream) {
-  if (dtype == kTypeF16) Launch<__half>(kind, args, stream);
-  else if (dtype == kTypeBf16) Launch<__nv_bfloat16>(kind, args, stream);
-  else throw InvalidArgument("routed products take F16 or BF16");
+  if (dtype != kTypeF16 && dtype != kTypeBf16) throw InvalidArgument("routed products take F16 or BF16");
+  if (TensorCoreProduct(kind, args)) LaunchTensorCoreProduct(kind, dtype, args, stream);
+  else if (dtype == kTypeF16) Launch<__half>(kind, args, stream);
+  else Launch<__nv_bfloat16>(kind, args, stream);
 }
 
 void LaunchRoutedSum(int32_t dtype, const RoutedSumArgs& args, cudaStream_t stream) {

@@ -1,0 +1,452 @@
+// Routed products on the tcgen05 tensor cores, for operands whose rows start
+// on 16-byte boundaries.
+//
+// A block owns one streaming multiprocessor and walks 128 x kWide output
+// tiles.  Warp 0 loads 64-deep slices into a ring of shared-memory stages by
+// TMA: token rows are gathered four at a time by their indices, so that no
+// ordered copy of the input is made.  One thread of warp 1 issues the matrix
+// instructions into one of two accumulators in tensor memory, and warps 2 to 5
+// round and store the other one meanwhile.
+//
+//   product:     A = rows of x (deep-major), B = W[e] as it lies (wide-major)
+//   transposed:  A = rows of x (deep-major), B = W[e]^T: W[e] as it lies (deep-major)
+//   weight grad: A = x^T, B = y: rows are the deep axis, both as they lie (wide-major)
+//
+// A tile's rows past its expert's last are computed from whatever the loads
+// bring and not stored.  In the weight gradient they would enter the sum: the
+// matrix warp zeroes them in shared memory, in both operands, so that a value
+// that is not finite stays with its own expert.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "engine.h"
+#include "layout.h"
+#include "routed.cuh"
+#include "routed.h"
+#include "tcgen05.cuh"
+
+namespace t0b {
+namespace {
+
+constexpr int kTileRows = 128, kDeep = 64, kTcThreads = 192;
+constexpr uint32_t kSwizzleRow = 128;                      // bytes of 64 16-bit values
+constexpr uint32_t kABytes = kTileRows * kSwizzleRow;      // one stage of A
+constexpr uint32_t kBlockBytes = kDeep * kSwizzleRow;      // 64 x 64 values
+constexpr int kMaxStages = 8;
+
+struct TcArgs {
+  CUtensorMap a, a_rows, b, b_rows;   // tiles, and single rows for gathering
+  const int32_t* rows;
+  const int32_t* offsets;
+  void* out;
+  int64_t entries;
+  int experts, top_k, inner, outer;
+  int gather_a, gather_b, bf16;
+};
+
+template <int kWide>
+struct TcShape {
+  static constexpr uint32_t kBBytes = kWide * kSwizzleRow;
+  static constexpr uint32_t kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = kWide == 256 ? 4 : kWide == 128 ? 6 : 8;
+  static constexpr uint32_t kRing = kStages * kStageBytes;
+};
+
+struct TcShared {
+  uint64_t full[kMaxStages], empty[kMaxStages], done[2], drained[2], drain;
+  uint32_t tmem;
+  volatile int failed;
+  int row_begin[kRouteMaxExperts + 1];
+  int tile_begin[kRouteMaxExperts + 1];
+};
+
+// Where a tile lies: output rows [m0, m0 + 128) of expert e (of its rows, or
+// of `inner` in the weight gradient), columns from n0.
+struct TcTile {
+  int e, m0, n0, rows;   // rows: what the expert has of the tile axis
+  int begin, count;      // the expert's first row and its rows
+};
+
+template <int kKind, int kWide>
+struct TcWalk {
+  const TcArgs& a;
+  const TcShared& s;
+  int e = 0;
+  __device__ TcWalk(const TcArgs& args, const TcShared& shared) : a(args), s(shared) {}
+  __device__ TcTile At(int tile) {
+    while (s.tile_begin[e + 1] <= tile) ++e;
+    TcTile t;
+    t.e = e;
+    t.begin = s.row_begin[e];
+    t.count = max(0, s.row_begin[e + 1] - t.begin);
+    t.rows = kKind == kProductWeightGrad ? a.inner : t.count;
+    const int local = tile - s.tile_begin[e], tiles_m = (t.rows + kTileRows - 1) / kTileRows;
+    t.m0 = local % tiles_m * kTileRows;
+    t.n0 = local / tiles_m * kWide;
+    return t;
+  }
+  __device__ int Slices(const TcTile& t) const {
+    const int deep = kKind == kProductWeightGrad ? t.count : kKind == kProduct ? a.inner : a.outer;
+    return (deep + kDeep - 1) / kDeep;
+  }
+};
+
+template <int kKind, int kWide>
+__global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant__ TcArgs a) {
+  using Shape = TcShape<kWide>;
+  extern __shared__ unsigned char tc_raw[];
+  __shared__ TcShared s;
+  const uint32_t ring = (SharedAddress(tc_raw) + 1023u) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int width = kKind == kProductTransposed ? a.inner : a.outer;
+  const int tiles_n = (width + kWide - 1) / kWide;
+  constexpr uint32_t kTmemColumns = 2 * kWide;
+
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SharedAddress(&s.tmem)),
+                 "r"(kTmemColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < Shape::kStages; ++i) {
+      BarrierInit(SharedAddress(&s.full[i]), 1);
+      BarrierInit(SharedAddress(&s.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      BarrierInit(SharedAddress(&s.done[i]), 1);
+      BarrierInit(SharedAddress(&s.drained[i]), 128);
+    }
+    BarrierInit(SharedAddress(&s.drain), 1);
+    s.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int e = tid; e <= a.experts; e += kTcThreads) {
+    s.row_begin[e] = static_cast<int>(RowBound(a.offsets[e], a.entries));
+  }
+  __syncthreads();
+  if (warp == 0) {   // tiles before each expert
+    int carry = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      const int e = e0 + lane;
+      int tiles = 0;
+      if (e < a.experts) {
+        const int rows = kKind == kProductWeightGrad ? a.inner : max(0, s.row_begin[e + 1] - s.row_begin[e]);
+        tiles = (rows + kTileRows - 1) / kTileRows * tiles_n;
+      }
+      int sum = tiles;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += other;
+      }
+      if (e < a.experts) s.tile_begin[e] = carry + sum - tiles;
+      carry += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) s.tile_begin[a.experts] = carry;
+  }
+  TmemFenceBefore();
+  __syncthreads();
+  TmemFenceAfter();
+  const uint32_t tmem = s.tmem;
+  const int tiles = s.tile_begin[a.experts];
+  TcWalk<kKind, kWide> walk(a, s);
+
+  if (warp == 0) {
+    // Loads.  `fill` counts the stages filled since the start.
+    uint32_t fill = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      const TcTile t = walk.At(tile);
+      const int slices = walk.Slices(t), last = t.begin + t.count - 1;
+      int rows[4];
+      if constexpr (kKind != kProductWeightGrad) {
+        if (a.gather_a != 0) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) rows[i] = a.rows[min(t.begin + t.m0 + lane * 4 + i, last)] / a.top_k;
+        }
+      }
+      // Column blocks of 64 that lie in the operand at all.
+      const int a_blocks = kKind == kProductWeightGrad ? min(2, (a.inner - t.m0 + 63) / 64) : 1;
+      const int b_blocks = min(kWide / 64, (width - t.n0 + 63) / 64);
+      const uint32_t bytes = (kKind == kProductWeightGrad ? a_blocks * kBlockBytes : kABytes) +
+                             (kKind == kProductTransposed ? Shape::kBBytes : b_blocks * kBlockBytes);
+      for (int k = 0; k < slices; ++k, ++fill) {
+        const int stage = static_cast<int>(fill % Shape::kStages);
+        const uint32_t a_smem = ring + stage * Shape::kStageBytes, b_smem = a_smem + kABytes;
+        const uint32_t full = SharedAddress(&s.full[stage]);
+        const int k0 = k * kDeep;
+        if constexpr (kKind == kProductWeightGrad) {
+          if (a.gather_a != 0 || a.gather_b != 0) {   // this slice's rows, 4 for each half warp's lane
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rows[i] = a.rows[min(t.begin + k0 + (lane & 15) * 4 + i, last)] / a.top_k;
+          }
+        }
+        if (fill >= Shape::kStages) {
+          ok = BarrierWait(SharedAddress(&s.empty[stage]), (fill / Shape::kStages + 1) & 1, &s.failed);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        }
+        if (lane == 0) BarrierExpect(full, bytes);
+        __syncwarp();
+        if constexpr (kKind == kProductWeightGrad) {
+          if (a.gather_a != 0) {
+            if ((lane >> 4) < a_blocks) {
+              LoadRows4(a_smem + (lane >> 4) * kBlockBytes + (lane & 15) * 512, &a.a_rows, full,
+                        t.m0 + (lane >> 4) * 64, rows[0], rows[1], rows[2], rows[3]);
+            }
+          } else if (lane < a_blocks) {
+            LoadTile2(a_smem + lane * kBlockBytes, &a.a, full, t.m0 + lane * 64, t.begin + k0);
+          }
+          if (a.gather_b != 0) {
+            for (int block = lane >> 4; block < b_blocks; block += 2) {
+              LoadRows4(b_smem + block * kBlockBytes + (lane & 15) * 512, &a.b_rows, full, t.n0 + block * 64, rows[0],
+                        rows[1], rows[2], rows[3]);
+            }
+          } else if (lane < b_blocks) {
+            LoadTile2(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, t.begin + k0);
+          }
+        } else {
+          if (a.gather_a != 0) {
+            LoadRows4(a_smem + lane * 512, &a.a_rows, full, k0, rows[0], rows[1], rows[2], rows[3]);
+          } else if (lane == 0) {
+            LoadTile2(a_smem, &a.a, full, k0, t.begin + t.m0);
+          }
+          if constexpr (kKind == kProduct) {
+            if (lane < b_blocks) LoadTile3(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, k0, t.e);
+          } else {
+            if (lane == 0) LoadTile3(b_smem, &a.b, full, k0, t.n0, t.e);
+          }
+        }
+      }
+    }
+    if (!ok) {   // given up: the copies in flight land before the block ends
+      const uint32_t pending = fill < Shape::kStages ? fill : Shape::kStages;
+      for (uint32_t f = fill - pending; f < fill; ++f) {
+        BarrierWait(SharedAddress(&s.full[f % Shape::kStages]), (f / Shape::kStages) & 1, nullptr);
+      }
+    }
+  } else if (warp == 1) {
+    // Matrix instructions, issued by lane 0.
+    constexpr uint32_t a_major = kKind == kProductWeightGrad ? 1u : 0u, b_major = kKind == kProductTransposed ? 0u : 1u;
+    const uint32_t format = a.bf16 != 0 ? 1u : 0u;
+    const uint32_t idesc = (1u << 4) | (format << 7) | (format << 10) | (a_major << 15) | (b_major << 16) |
+                           ((kWide >> 3) << 17) | ((kTileRows >> 4) << 24);
+    uint32_t fill = 0, turn = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      const TcTile t = walk.At(tile);
+      const int slices = walk.Slices(t);
+      if (slices == 0) continue;
+      const uint32_t buffer = turn & 1;
+      if (turn >= 2) ok = BarrierWait(SharedAddress(&s.drained[buffer]), ((turn >> 1) + 1) & 1, &s.failed);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      TmemFenceAfter();
+      const uint32_t accumulator = tmem + buffer * kWide;
+      for (int k = 0; k < slices; ++k, ++fill) {
+        const int stage = static_cast<int>(fill % Shape::kStages);
+        ok = BarrierWait(SharedAddress(&s.full[stage]), (fill / Shape::kStages) & 1, &s.failed);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        const uint32_t a_smem = ring + stage * Shape::kStageBytes, b_smem = a_smem + kABytes;
+        if constexpr (kKind == kProductWeightGrad) {
+          const int valid = t.count - k * kDeep;
+          if (valid < kDeep) {   // rows of the next expert: zero, in every column block of both operands
+            const int blocks = 2 + kWide / 64, chunks = (kDeep - valid) * 8;
+            for (int i = lane; i < blocks * chunks; i += 32) {
+              const uint32_t at = a_smem + (i / chunks) * kBlockBytes + valid * kSwizzleRow + (i % chunks) * 16;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        }
+        TmemFenceAfter();
+        if (lane == 0) {
+#pragma unroll
+          for (int step = 0; step < kDeep / 16; ++step) {
+            const uint64_t left = a_major ? WideMajor(a_smem + step * 16 * kSwizzleRow, kBlockBytes)
+                                          : DeepMajor(a_smem + step * 32);
+            const uint64_t right = b_major ? WideMajor(b_smem + step * 16 * kSwizzleRow, kBlockBytes)
+                                           : DeepMajor(b_smem + step * 32);
+            MmaHalf(accumulator, left, right, idesc, k == 0 && step == 0 ? 0u : 1u);
+          }
+          MmaCommit(SharedAddress(&s.empty[stage]));
+          if (k == slices - 1) MmaCommit(SharedAddress(&s.done[buffer]));
+        }
+        __syncwarp();
+      }
+      ++turn;
+    }
+    if (!ok) {
+      if (lane == 0) MmaCommit(SharedAddress(&s.drain));
+      BarrierWait(SharedAddress(&s.drain), 0, nullptr);
+    }
+  } else {
+    // Rounding and stores: a thread has one row of the tile.
+    const int quarter = warp & 3;
+    uint16_t* out = static_cast<uint16_t*>(a.out);
+    uint32_t turn = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+      const TcTile t = walk.At(tile);
+      const bool empty = walk.Slices(t) == 0;
+      const uint32_t buffer = turn & 1;
+      if (!empty) {
+        ok = ok && BarrierWait(SharedAddress(&s.done[buffer]), (turn >> 1) & 1, &s.failed);
+        TmemFenceAfter();
+      }
+      const int m = t.m0 + quarter * 32 + lane;
+      const bool stored = m < t.rows;
+      uint16_t* row = out + (kKind == kProductWeightGrad ? static_cast<int64_t>(t.e) * a.inner + m
+                                                         : static_cast<int64_t>(t.begin) + m) * width;
+      const uint32_t source = tmem + buffer * kWide + (static_cast<uint32_t>(quarter * 32) << 16);
+      const int columns = min(kWide, width - t.n0);
+      for (int c = 0; c < columns; c += 32) {
+        uint32_t r[32];
+        if (!__all_sync(0xffffffffu, ok)) {   // a wait gave up: no partial sums
+          ok = false;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0x7fc00000u;
+        } else if (empty) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        } else {
+          TmemLoad(source + c, r);
+          TmemLoadWait();
+        }
+        if (stored) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (t.n0 + c + q * 8 < width) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float lo = __uint_as_float(r[q * 8 + 2 * i]), hi = __uint_as_float(r[q * 8 + 2 * i + 1]);
+                w[i] = a.bf16 != 0 ? Pack2<__nv_bfloat16>(lo, hi) : Pack2<__half>(lo, hi);
+              }
+              *reinterpret_cast<uint4*>(row + t.n0 + c + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+      if (!empty) {
+        TmemFenceBefore();
+        BarrierArrive(SharedAddress(&s.drained[buffer]));
+        ++turn;
+      }
+    }
+    if constexpr (kKind != kProductWeightGrad) {   // rows without an expert
+      const int64_t from = int64_t{s.row_begin[a.experts]} * width / 8, to = a.entries * width / 8;
+      uint4* zeros = reinterpret_cast<uint4*>(a.out);
+      for (int64_t i = from + blockIdx.x * 128 + (tid - 64); i < to; i += int64_t{gridDim.x} * 128) {
+        zeros[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  TmemFenceBefore();
+  __syncthreads();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
+  }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled Encoder() {
+  static const EncodeTiled function = [] {
+    void* entry = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    Check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &found), "tensor map entry point");
+    if (found != cudaDriverEntryPointSuccess || entry == nullptr) {
+      throw std::runtime_error("the driver has no cuTensorMapEncodeTiled");
+    }
+    return reinterpret_cast<EncodeTiled>(entry);
+  }();
+  return function;
+}
+
+// Map of a 16-bit operand [depth, rows, columns] (depth 0: two dimensions)
+// with boxes of 64 columns and `box` rows, 128-byte swizzled.
+void Encode(CUtensorMap* map, bool bf16, const void* data, int64_t columns, int64_t rows, int64_t depth,
+            int64_t row_stride, int64_t depth_stride, int box) {
+  const cuuint64_t sizes[3] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows),
+                               static_cast<cuuint64_t>(depth)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_stride) * 2, static_cast<cuuint64_t>(depth_stride) * 2};
+  const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box), 1}, steps[3] = {1, 1, 1};
+  const CUresult status = Encoder()(
+      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth != 0 ? 3 : 2,
+      const_cast<void*>(data), sizes, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (status != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed");
+}
+
+template <int kKind, int kWide>
+void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStream_t stream) {
+  using Shape = TcShape<kWide>;
+  TcArgs a{};
+  const int x_width = kKind == kProductTransposed ? p.outer : p.inner;
+  if (p.gather_x != 0) Encode(&a.a_rows, bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, 1);
+  else Encode(&a.a, bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kTileRows);
+  if constexpr (kKind == kProductWeightGrad) {
+    if (p.gather_w != 0) Encode(&a.b_rows, bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, 1);
+    else Encode(&a.b, bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
+  } else {
+    Encode(&a.b, bf16, p.w, p.outer, p.inner, p.experts, p.outer, int64_t{p.inner} * p.outer,
+           kKind == kProduct ? kDeep : kWide);
+  }
+  a.rows = p.rows;
+  a.offsets = p.offsets;
+  a.out = p.out;
+  a.entries = p.entries;
+  a.experts = p.experts;
+  a.top_k = p.top_k;
+  a.inner = p.inner;
+  a.outer = p.outer;
+  a.gather_a = p.gather_x;
+  a.gather_b = p.gather_w;
+  a.bf16 = bf16 ? 1 : 0;
+  constexpr int smem = static_cast<int>(Shape::kRing) + 1024;
+  Check(cudaFuncSetAttribute(TcProduct<kKind, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+        "routed product shared memory");
+  const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(tiles, sms)));
+  TcProduct<kKind, kWide><<<grid, kTcThreads, smem, stream>>>(a);
+  Check(cudaGetLastError(), "routed product launch");
+  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+}
+
+template <int kKind>
+void ByWidth(const ProductArgs& p, bool bf16, cudaStream_t stream) {
+  const int sms = RoutedSmCount();
+  const int64_t width = kKind == kProductTransposed ? p.inner : p.outer;
+  // Row tiles: the experts' row counts stay on the device, so at most one
+  // partial tile per expert (or per row) on top of the whole ones.
+  const int64_t row_tiles = kKind == kProductWeightGrad
+                                ? int64_t{p.experts} * ((p.inner + kTileRows - 1) / kTileRows)
+                                : p.entries / kTileRows + std::min<int64_t>(p.experts, p.entries);
+  const auto tiles = [&](int wide) { return row_tiles * ((width + wide - 1) / wide); };
+  if (tiles(256) >= sms) LaunchTc<kKind, 256>(p, bf16, tiles(256), sms, stream);
+  else if (tiles(128) >= sms) LaunchTc<kKind, 128>(p, bf16, tiles(128), sms, stream);
+  else LaunchTc<kKind, 64>(p, bf16, tiles(64), sms, stream);
+}
+
+}  // namespace
+
+// Every operand row starts on a 16-byte boundary and no tile index passes 32 bits.
+bool TensorCoreProduct(int kind, const ProductArgs& p) {
+  const auto aligned = [](const void* data) { return reinterpret_cast<uintptr_t>(data) % 16 == 0; };
+  const int64_t width = kind == kProductTransposed ? p.inner : p.outer;
+  const int64_t rows = kind == kProductWeightGrad ? int64_t{p.experts} * (p.inner + kTileRows) : p.entries + int64_t{p.experts} * kTileRows;
+  return p.entries > 0 && p.inner % 8 == 0 && p.outer % 8 == 0 && p.x_stride % 8 == 0 &&
+         (kind != kProductWeightGrad || p.w_stride % 8 == 0) && aligned(p.x) && aligned(p.w) && aligned(p.out) &&
+         rows / kTileRows * ((width + 63) / 64) < (int64_t{1} << 31);
+}
+
+void LaunchTensorCoreProduct(int kind, int32_t dtype, const ProductArgs& args, cudaStream_t stream) {
+  const bool bf16 = dtype == kTypeBf16;
+  if (kind == kProduct) ByWidth<kProduct>(args, bf16, stream);
+  else if (kind == kProductTransposed) ByWidth<kProductTransposed>(args, bf16, stream);
+  else ByWidth<kProductWeightGrad>(args, bf16, stream);
+}
+
+}  // namespace t0b

@@ -66,6 +66,9 @@ struct ProductArgs {
 
 enum ProductKind : int { kProduct = 0, kProductTransposed = 1, kProductWeightGrad = 2 };
 void LaunchProduct(int kind, int32_t dtype, const ProductArgs& args, cudaStream_t stream);
+// The tensor-core kernel of LaunchProduct, where it takes the operands.
+bool TensorCoreProduct(int kind, const ProductArgs& args);
+void LaunchTensorCoreProduct(int kind, int32_t dtype, const ProductArgs& args, cudaStream_t stream);
 
 // out[t] = sum over the token's slots of y[positions[t, slot]].
 struct RoutedSumArgs {

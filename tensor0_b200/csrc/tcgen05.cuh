@@ -1,0 +1,118 @@
+// sm_100a building blocks of the routed products: mbarriers with bounded
+// waits, TMA tile and row-gather loads, tcgen05 instructions and descriptors.
+#pragma once
+
+#include <cstdint>
+
+namespace t0b {
+
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;   // a wait gives up after two seconds
+
+__device__ __forceinline__ uint32_t SharedAddress(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ void BarrierInit(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void BarrierArrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void BarrierExpect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ bool BarrierTry(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ unsigned long long Nanoseconds() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Wait for a phase.  False if it did not come within the limit, or another
+// role of the block has given up (`failed`, null to ignore it).
+__device__ __forceinline__ bool BarrierWait(uint32_t bar, uint32_t parity, volatile int* failed) {
+  if (BarrierTry(bar, parity)) return true;
+  const unsigned long long start = Nanoseconds();
+  while (!BarrierTry(bar, parity)) {
+    if (failed != nullptr && *failed != 0) return false;
+    if (Nanoseconds() - start > kWaitLimitNs) {
+      if (failed != nullptr) *failed = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void LoadTile2(uint32_t dst, const void* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+
+__device__ __forceinline__ void LoadTile3(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// Four rows of a matrix whose map has a box one row high.
+__device__ __forceinline__ void LoadRows4(uint32_t dst, const void* map, uint32_t bar, int x, int r0, int r1, int r2,
+                                          int r3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+
+// Shared-memory matrix descriptors of 128-byte swizzled tiles of 16-bit values.
+// Deep-major (K-major): rows of 64 deep values, 8-row atoms 1024 bytes apart.
+// Wide-major (MN-major): 64 neighbours of one deep index per 128 bytes, 8 deep
+// indices per 1024-byte atom, blocks of 64 neighbours `block` bytes apart.
+__device__ __forceinline__ uint64_t DeepMajor(uint32_t address) {
+  return static_cast<uint64_t>((address >> 4) & 0x3FFF) | (uint64_t{1} << 16) | (uint64_t{1024 >> 4} << 32) |
+         (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+
+__device__ __forceinline__ uint64_t WideMajor(uint32_t address, uint32_t block) {
+  return static_cast<uint64_t>((address >> 4) & 0x3FFF) | (static_cast<uint64_t>(block >> 4) << 16) |
+         (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+
+__device__ __forceinline__ void MmaHalf(uint32_t tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+      ::"r"(tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+__device__ __forceinline__ void MmaCommit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void TmemFenceBefore() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void TmemFenceAfter() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void TmemLoadWait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 32 columns of the warp's 32 tensor-memory lanes; TmemLoadWait before use.
+__device__ __forceinline__ void TmemLoad(uint32_t address, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(address));
+}
+
+}  // namespace t0b
