@@ -3,10 +3,13 @@
 //
 // A block owns one streaming multiprocessor and walks 128 x kWide output
 // tiles.  Warp 0 loads 64-deep slices into a ring of shared-memory stages by
-// TMA: token rows are gathered four at a time by their indices, so that no
-// ordered copy of the input is made.  One thread of warp 1 issues the matrix
-// instructions into one of two accumulators in tensor memory, and warps 2 to 5
-// round and store the other one meanwhile.
+// TMA.  One thread of warp 1 issues the matrix instructions into one of two
+// accumulators in tensor memory, and warps 2 to 5 round and store the other one
+// meanwhile.  Where rows are gathered, warps 6 to 9 copy them by their indices
+// with 16-byte asynchronous copies, straight from the token rows: no ordered
+// copy of the input is made.  (TMA's own four-row gather was measured at about
+// 100 cycles an instruction, 512 bytes each: 1.8 us a slice against 0.28 us of
+// matrix instructions.)
 //
 //   product:     A = rows of x (deep-major), B = W[e] as it lies (wide-major)
 //   transposed:  A = rows of x (deep-major), B = W[e]^T: W[e] as it lies (deep-major)
@@ -29,14 +32,18 @@
 namespace t0b {
 namespace {
 
-constexpr int kTileRows = 128, kDeep = 64, kTcThreads = 192;
+constexpr int kTileRows = 128, kDeep = 64;
+constexpr int kTcThreads = 192, kGatherThreads = 128;      // roles; copying threads where rows are gathered
 constexpr uint32_t kSwizzleRow = 128;                      // bytes of 64 16-bit values
 constexpr uint32_t kABytes = kTileRows * kSwizzleRow;      // one stage of A
 constexpr uint32_t kBlockBytes = kDeep * kSwizzleRow;      // 64 x 64 values
 constexpr int kMaxStages = 8;
+constexpr uint32_t kStagingBytes = 32 * kSwizzleRow;       // of one storing warp
 
 struct TcArgs {
-  CUtensorMap a, a_rows, b, b_rows;   // tiles, and single rows for gathering
+  CUtensorMap a, b;
+  const uint16_t *a_data, *b_data;   // gathered operands
+  int64_t a_rows, a_stride, b_rows, b_stride;
   const int32_t* rows;
   const int32_t* offsets;
   void* out;
@@ -92,8 +99,15 @@ struct TcWalk {
   }
 };
 
-template <int kKind, int kWide>
-__global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant__ TcArgs a) {
+// Copies 16 bytes of row `r` into a swizzled tile of 128-byte rows, chunk c of
+// eight; zeros if !inside.
+__device__ __forceinline__ void CopyChunk(uint32_t tile, int r, int c, const uint16_t* source, bool inside) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+               ::"r"(tile + r * kSwizzleRow + ((c ^ (r & 7)) << 4)), "l"(source), "r"(inside ? 16 : 0) : "memory");
+}
+
+template <int kKind, int kWide, bool kGather>
+__global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1) TcProduct(const __grid_constant__ TcArgs a) {
   using Shape = TcShape<kWide>;
   extern __shared__ unsigned char tc_raw[];
   __shared__ TcShared s;
@@ -110,7 +124,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
   }
   if (tid == 0) {
     for (int i = 0; i < Shape::kStages; ++i) {
-      BarrierInit(SharedAddress(&s.full[i]), 1);
+      BarrierInit(SharedAddress(&s.full[i]), 1 + (kGather ? kGatherThreads : 0));
       BarrierInit(SharedAddress(&s.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -121,7 +135,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
     s.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int e = tid; e <= a.experts; e += kTcThreads) {
+  for (int e = tid; e <= a.experts; e += blockDim.x) {
     s.row_begin[e] = static_cast<int>(RowBound(a.offsets[e], a.entries));
   }
   __syncthreads();
@@ -158,30 +172,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
     bool ok = true;
     for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
       const TcTile t = walk.At(tile);
-      const int slices = walk.Slices(t), last = t.begin + t.count - 1;
-      int rows[4];
-      if constexpr (kKind != kProductWeightGrad) {
-        if (a.gather_a != 0) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) rows[i] = a.rows[min(t.begin + t.m0 + lane * 4 + i, last)] / a.top_k;
-        }
-      }
+      const int slices = walk.Slices(t);
       // Column blocks of 64 that lie in the operand at all.
       const int a_blocks = kKind == kProductWeightGrad ? min(2, (a.inner - t.m0 + 63) / 64) : 1;
       const int b_blocks = min(kWide / 64, (width - t.n0 + 63) / 64);
-      const uint32_t bytes = (kKind == kProductWeightGrad ? a_blocks * kBlockBytes : kABytes) +
-                             (kKind == kProductTransposed ? Shape::kBBytes : b_blocks * kBlockBytes);
+      const uint32_t a_bytes = kKind == kProductWeightGrad ? a_blocks * kBlockBytes : kABytes;
+      const uint32_t b_bytes = kKind == kProductTransposed ? Shape::kBBytes : b_blocks * kBlockBytes;
+      const bool load_a = !kGather || a.gather_a == 0, load_b = !kGather || a.gather_b == 0;
+      const uint32_t bytes = (load_a ? a_bytes : 0) + (load_b ? b_bytes : 0);
       for (int k = 0; k < slices; ++k, ++fill) {
         const int stage = static_cast<int>(fill % Shape::kStages);
         const uint32_t a_smem = ring + stage * Shape::kStageBytes, b_smem = a_smem + kABytes;
         const uint32_t full = SharedAddress(&s.full[stage]);
         const int k0 = k * kDeep;
-        if constexpr (kKind == kProductWeightGrad) {
-          if (a.gather_a != 0 || a.gather_b != 0) {   // this slice's rows, 4 for each half warp's lane
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rows[i] = a.rows[min(t.begin + k0 + (lane & 15) * 4 + i, last)] / a.top_k;
-          }
-        }
         if (fill >= Shape::kStages) {
           ok = BarrierWait(SharedAddress(&s.empty[stage]), (fill / Shape::kStages + 1) & 1, &s.failed);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -189,28 +192,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
         if (lane == 0) BarrierExpect(full, bytes);
         __syncwarp();
         if constexpr (kKind == kProductWeightGrad) {
-          if (a.gather_a != 0) {
-            if ((lane >> 4) < a_blocks) {
-              LoadRows4(a_smem + (lane >> 4) * kBlockBytes + (lane & 15) * 512, &a.a_rows, full,
-                        t.m0 + (lane >> 4) * 64, rows[0], rows[1], rows[2], rows[3]);
-            }
-          } else if (lane < a_blocks) {
+          if (load_a && lane < a_blocks) {
             LoadTile2(a_smem + lane * kBlockBytes, &a.a, full, t.m0 + lane * 64, t.begin + k0);
           }
-          if (a.gather_b != 0) {
-            for (int block = lane >> 4; block < b_blocks; block += 2) {
-              LoadRows4(b_smem + block * kBlockBytes + (lane & 15) * 512, &a.b_rows, full, t.n0 + block * 64, rows[0],
-                        rows[1], rows[2], rows[3]);
-            }
-          } else if (lane < b_blocks) {
+          if (load_b && lane < b_blocks) {
             LoadTile2(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, t.begin + k0);
           }
         } else {
-          if (a.gather_a != 0) {
-            LoadRows4(a_smem + lane * 512, &a.a_rows, full, k0, rows[0], rows[1], rows[2], rows[3]);
-          } else if (lane == 0) {
-            LoadTile2(a_smem, &a.a, full, k0, t.begin + t.m0);
-          }
+          if (load_a && lane == 0) LoadTile2(a_smem, &a.a, full, k0, t.begin + t.m0);
           if constexpr (kKind == kProduct) {
             if (lane < b_blocks) LoadTile3(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, k0, t.e);
           } else {
@@ -247,6 +236,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
         ok = BarrierWait(SharedAddress(&s.full[stage]), (fill / Shape::kStages) & 1, &s.failed);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         const uint32_t a_smem = ring + stage * Shape::kStageBytes, b_smem = a_smem + kABytes;
+        if constexpr (kGather) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         if constexpr (kKind == kProductWeightGrad) {
           const int valid = t.count - k * kDeep;
           if (valid < kDeep) {   // rows of the next expert: zero, in every column block of both operands
@@ -280,9 +270,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
       if (lane == 0) MmaCommit(SharedAddress(&s.drain));
       BarrierWait(SharedAddress(&s.drain), 0, nullptr);
     }
-  } else {
-    // Rounding and stores: a thread has one row of the tile.
+  } else if (warp < 6) {
+    // Rounding and stores: a warp has 32 rows of the tile, 64 columns at a time.
     const int quarter = warp & 3;
+    const uint32_t staging = ring + Shape::kRing + quarter * kStagingBytes;
     uint16_t* out = static_cast<uint16_t*>(a.out);
     uint32_t turn = 0;
     bool ok = true;
@@ -294,37 +285,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
         ok = ok && BarrierWait(SharedAddress(&s.done[buffer]), (turn >> 1) & 1, &s.failed);
         TmemFenceAfter();
       }
-      const int m = t.m0 + quarter * 32 + lane;
-      const bool stored = m < t.rows;
-      uint16_t* row = out + (kKind == kProductWeightGrad ? static_cast<int64_t>(t.e) * a.inner + m
-                                                         : static_cast<int64_t>(t.begin) + m) * width;
       const uint32_t source = tmem + buffer * kWide + (static_cast<uint32_t>(quarter * 32) << 16);
-      const int columns = min(kWide, width - t.n0);
-      for (int c = 0; c < columns; c += 32) {
-        uint32_t r[32];
+      const int columns = min(kWide, width - t.n0), m0 = t.m0 + quarter * 32;
+      uint16_t* rows = out + (kKind == kProductWeightGrad ? static_cast<int64_t>(t.e) * a.inner
+                                                          : static_cast<int64_t>(t.begin)) * width;
+      for (int c = 0; c < columns; c += 64) {
+        uint32_t r[2][32], w[32];
         if (!__all_sync(0xffffffffu, ok)) {   // a wait gave up: no partial sums
           ok = false;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0x7fc00000u;
+          for (int i = 0; i < 32; ++i) w[i] = 0x7fff7fffu;
         } else if (empty) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0u;
+          for (int i = 0; i < 32; ++i) w[i] = 0u;
         } else {
-          TmemLoad(source + c, r);
+          TmemLoad(source + c, r[0]);
+          TmemLoad(source + c + 32, r[1]);
           TmemLoadWait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float lo = __uint_as_float(r[i >> 4][(2 * i) & 31]), hi = __uint_as_float(r[i >> 4][(2 * i + 1) & 31]);
+            w[i] = a.bf16 != 0 ? Pack2<__nv_bfloat16>(lo, hi) : Pack2<__half>(lo, hi);
+          }
         }
-        if (stored) {
+        // Through shared memory, so that a store writes whole 128-byte rows.
+        __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (t.n0 + c + q * 8 < width) {
-              uint32_t w[4];
+        for (int q = 0; q < 8; ++q) {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                       ::"r"(staging + lane * kSwizzleRow + ((q ^ (lane & 7)) << 4)), "r"(w[4 * q]), "r"(w[4 * q + 1]),
+                       "r"(w[4 * q + 2]), "r"(w[4 * q + 3]) : "memory");
+        }
+        __syncwarp();
+        const int column = t.n0 + c + (lane & 7) * 8;
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float lo = __uint_as_float(r[q * 8 + 2 * i]), hi = __uint_as_float(r[q * 8 + 2 * i + 1]);
-                w[i] = a.bf16 != 0 ? Pack2<__nv_bfloat16>(lo, hi) : Pack2<__half>(lo, hi);
-              }
-              *reinterpret_cast<uint4*>(row + t.n0 + c + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+        for (int i = 0; i < 8; ++i) {
+          const int row = i * 4 + (lane >> 3);
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(staging + row * kSwizzleRow + (((lane & 7) ^ (row & 7)) << 4)) : "memory");
+          if (m0 + row < t.rows && column < width) {
+            *reinterpret_cast<uint4*>(rows + static_cast<int64_t>(m0 + row) * width + column) = v;
           }
         }
       }
@@ -341,6 +343,69 @@ __global__ void __launch_bounds__(kTcThreads, 1) TcProduct(const __grid_constant
         zeros[i] = make_uint4(0, 0, 0, 0);
       }
     }
+  } else if constexpr (kGather) {
+    // Gathered rows: eight threads copy 128 bytes of a row, a thread the same
+    // chunk of rows r0, r0 + 16, ...  A thread's arrival at the stage's barrier
+    // follows its copies by itself; the matrix warp then orders them before the
+    // tensor cores' reads.
+    const int g = tid - kTcThreads, c = g & 7, r0 = g >> 3;
+    uint32_t fill = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      const TcTile t = walk.At(tile);
+      const int slices = walk.Slices(t), last = t.begin + t.count - 1;
+      const uint16_t* source[8];   // the tile's rows (products)
+      int64_t next[4];             // the next slice's token rows (weight gradient)
+      auto slice_rows = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[i] = a.rows[min(t.begin + k * kDeep + r0 + 16 * i, last)] / a.top_k;
+      };
+      if constexpr (kKind != kProductWeightGrad) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int64_t row = a.rows[min(t.begin + t.m0 + r0 + 16 * i, last)] / a.top_k;
+          source[i] = a.a_data + (row >= 0 && row < a.a_rows ? row : 0) * a.a_stride + c * 8;
+        }
+      } else if (slices > 0) {
+        slice_rows(0);
+      }
+      for (int k = 0; k < slices; ++k, ++fill) {
+        const int stage = static_cast<int>(fill % Shape::kStages);
+        const uint32_t a_smem = ring + stage * Shape::kStageBytes, b_smem = a_smem + kABytes;
+        if (fill >= Shape::kStages) {
+          ok = BarrierWait(SharedAddress(&s.empty[stage]), (fill / Shape::kStages + 1) & 1, &s.failed);
+          if (!ok) break;
+        }
+        if constexpr (kKind != kProductWeightGrad) {
+          const int deep = kKind == kProduct ? a.inner : a.outer;
+          const bool inside = k * kDeep + c * 8 < deep;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) CopyChunk(a_smem, r0 + 16 * i, c, inside ? source[i] + k * kDeep : a.a_data, inside);
+        } else {
+          int64_t row[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) row[i] = next[i];
+          auto copy = [&](uint32_t tile_smem, const uint16_t* data, int64_t rows, int64_t stride, int column, int columns,
+                          int blocks) {
+            for (int block = 0; block < blocks; ++block) {
+              const int at = column + block * 64 + c * 8;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const bool inside = at < columns && row[i] >= 0 && row[i] < rows;
+                CopyChunk(tile_smem + block * kBlockBytes, r0 + 16 * i, c, inside ? data + row[i] * stride + at : data,
+                          inside);
+              }
+            }
+          };
+          if (a.gather_a != 0) copy(a_smem, a.a_data, a.a_rows, a.a_stride, t.m0, a.inner, 2);
+          if (a.gather_b != 0) copy(b_smem, a.b_data, a.b_rows, a.b_stride, t.n0, a.outer, kWide / 64);
+          if (k + 1 < slices) slice_rows(k + 1);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];"
+                     ::"r"(SharedAddress(&s.full[stage])) : "memory");
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   TmemFenceBefore();
   __syncthreads();
@@ -381,20 +446,26 @@ void Encode(CUtensorMap* map, bool bf16, const void* data, int64_t columns, int6
   if (status != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed");
 }
 
-template <int kKind, int kWide>
+template <int kKind, int kWide, bool kGather>
 void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStream_t stream) {
   using Shape = TcShape<kWide>;
   TcArgs a{};
   const int x_width = kKind == kProductTransposed ? p.outer : p.inner;
-  if (p.gather_x != 0) Encode(&a.a_rows, bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, 1);
-  else Encode(&a.a, bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kTileRows);
+  if (p.gather_x == 0) {
+    Encode(&a.a, bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kTileRows);
+  }
   if constexpr (kKind == kProductWeightGrad) {
-    if (p.gather_w != 0) Encode(&a.b_rows, bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, 1);
-    else Encode(&a.b, bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
+    if (p.gather_w == 0) Encode(&a.b, bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
   } else {
     Encode(&a.b, bf16, p.w, p.outer, p.inner, p.experts, p.outer, int64_t{p.inner} * p.outer,
            kKind == kProduct ? kDeep : kWide);
   }
+  a.a_data = static_cast<const uint16_t*>(p.x);
+  a.a_rows = p.x_rows;
+  a.a_stride = p.x_stride;
+  a.b_data = static_cast<const uint16_t*>(p.w);
+  a.b_rows = p.w_rows;
+  a.b_stride = p.w_stride;
   a.rows = p.rows;
   a.offsets = p.offsets;
   a.out = p.out;
@@ -406,11 +477,11 @@ void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStrea
   a.gather_a = p.gather_x;
   a.gather_b = p.gather_w;
   a.bf16 = bf16 ? 1 : 0;
-  constexpr int smem = static_cast<int>(Shape::kRing) + 1024;
-  Check(cudaFuncSetAttribute(TcProduct<kKind, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+  constexpr int smem = static_cast<int>(Shape::kRing + 4 * kStagingBytes) + 1024;
+  Check(cudaFuncSetAttribute(TcProduct<kKind, kWide, kGather>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
         "routed product shared memory");
   const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(tiles, sms)));
-  TcProduct<kKind, kWide><<<grid, kTcThreads, smem, stream>>>(a);
+  TcProduct<kKind, kWide, kGather><<<grid, kTcThreads + (kGather ? kGatherThreads : 0), smem, stream>>>(a);
   Check(cudaGetLastError(), "routed product launch");
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
 }
@@ -425,9 +496,14 @@ void ByWidth(const ProductArgs& p, bool bf16, cudaStream_t stream) {
                                 ? int64_t{p.experts} * ((p.inner + kTileRows - 1) / kTileRows)
                                 : p.entries / kTileRows + std::min<int64_t>(p.experts, p.entries);
   const auto tiles = [&](int wide) { return row_tiles * ((width + wide - 1) / wide); };
-  if (tiles(256) >= sms) LaunchTc<kKind, 256>(p, bf16, tiles(256), sms, stream);
-  else if (tiles(128) >= sms) LaunchTc<kKind, 128>(p, bf16, tiles(128), sms, stream);
-  else LaunchTc<kKind, 64>(p, bf16, tiles(64), sms, stream);
+  const auto launch = [&](auto wide) {
+    constexpr int kWide = decltype(wide)::value;
+    if (p.gather_x != 0 || p.gather_w != 0) LaunchTc<kKind, kWide, true>(p, bf16, tiles(kWide), sms, stream);
+    else LaunchTc<kKind, kWide, false>(p, bf16, tiles(kWide), sms, stream);
+  };
+  if (tiles(256) >= sms) launch(std::integral_constant<int, 256>{});
+  else if (tiles(128) >= sms) launch(std::integral_constant<int, 128>{});
+  else launch(std::integral_constant<int, 64>{});
 }
 
 }  // namespace

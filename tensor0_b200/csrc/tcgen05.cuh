@@ -1,5 +1,5 @@
 // sm_100a building blocks of the routed products: mbarriers with bounded
-// waits, TMA tile and row-gather loads, tcgen05 instructions and descriptors.
+// waits, TMA tile loads, tcgen05 instructions and descriptors.
 #pragma once
 
 #include <cstdint>
@@ -63,15 +63,6 @@ __device__ __forceinline__ void LoadTile3(uint32_t dst, const void* map, uint32_
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
       ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-
-// Four rows of a matrix whose map has a box one row high.
-__device__ __forceinline__ void LoadRows4(uint32_t dst, const void* map, uint32_t bar, int x, int r0, int r1, int r2,
-                                          int r3) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
-      "[%1, {%3, %4, %5, %6, %7}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 
 // Shared-memory matrix descriptors of 128-byte swizzled tiles of 16-bit values.

@@ -273,6 +273,10 @@ PRODUCTS = [
     (40, 6, 2, 40, 19, 0.2, None),
     (40, 6, 2, 21, 48, 0.2, None),
     (513, 3, 2, 1032, 520, 0.05, None),
+    (300, 30, 2, 72, 640, 0.1, None),          # enough tiles for the wider ones, forward and transposed
+    (300, 30, 2, 640, 72, 0.1, None),
+    (700, 40, 2, 72, 1032, 0.1, None),
+    (700, 40, 2, 1032, 72, 0.1, None),
 ]
 
 
