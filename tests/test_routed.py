@@ -546,7 +546,8 @@ def test_checkpoint_groups_that_are_not_finite_or_tiny():
 @pytest.mark.parametrize("gather", [False, True])
 @pytest.mark.parametrize("tokens, experts, top_k, inner, outer, group, absent",
                          [(0, 2, 1, 32, 8, 32, 0.0), (1, 4, 2, 64, 1, 64, 0.0), (1, 16, 8, 512, 100, 128, 0.3),
-                          (7, 3, 2, 96, 33, 32, 0.2), (40, 2, 2, 256, 24, 64, 0.0), (13, 20, 4, 1152, 257, 128, 0.1)])
+                          (7, 3, 2, 96, 33, 32, 0.2), (40, 2, 2, 256, 24, 64, 0.0), (13, 20, 4, 1152, 257, 128, 0.1),
+                          (3, 5, 2, 4256, 40, 32, 0.0), (5, 4, 2, 8320, 48, 64, 0.0)])
 def test_routed_matvec(tokens, experts, top_k, inner, outer, group, absent, gather, dtype):
     kind, unit, tiny = HALF[dtype]
     host, r = make_routing(tokens, experts, top_k, 15, absent)
