@@ -289,8 +289,7 @@ void Launch(const MatvecArgs& a, cudaStream_t stream) {
   const int rows = static_cast<int>(std::min<int64_t>(8, a.entries)), stride = MvStride(a.inner);
   const int smem = rows * (stride * 16 + (stride - 4) * 8 / kGroup * 4);
   const bool vector = a.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
-  Check(cudaFuncSetAttribute(Matvec<T, kGroup, kParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-        "4-bit product shared memory");
+  AllowShared<Matvec<T, kGroup, kParts>>(smem);
   Matvec<T, kGroup, kParts><<<static_cast<unsigned>(blocks), kMvThreads, smem, stream>>>(a, row_blocks, rows, vector);
   Check(cudaGetLastError(), "4-bit product launch");
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);

@@ -478,8 +478,7 @@ void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStrea
   a.gather_b = p.gather_w;
   a.bf16 = bf16 ? 1 : 0;
   constexpr int smem = static_cast<int>(Shape::kRing + 4 * kStagingBytes) + 1024;
-  Check(cudaFuncSetAttribute(TcProduct<kKind, kWide, kGather>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-        "routed product shared memory");
+  AllowShared<TcProduct<kKind, kWide, kGather>>(smem);
   const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(tiles, sms)));
   TcProduct<kKind, kWide, kGather><<<grid, kTcThreads + (kGather ? kGatherThreads : 0), smem, stream>>>(a);
   Check(cudaGetLastError(), "routed product launch");

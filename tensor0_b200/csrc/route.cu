@@ -419,8 +419,7 @@ void Route(const RouteArgs& a, cudaStream_t stream) {
   if (a.tokens <= kOneBlockTokens) {
     const unsigned warps = static_cast<unsigned>(std::min<int64_t>(32, std::max<int64_t>(1, a.tokens)));
     const std::size_t smem = (bins + warps * bins) * sizeof(int);
-    Check(cudaFuncSetAttribute(RouteOneBlock<T, V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(smem)), "router shared memory");
+    AllowShared<RouteOneBlock<T, V>>(static_cast<int>(smem));
     RouteOneBlock<T, V><<<1, warps * 32, smem, stream>>>(a);
     Check(cudaGetLastError(), "router launch");
     g_kernel_launches.fetch_add(1, std::memory_order_relaxed);

@@ -4,7 +4,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdint>
+
+#include "engine.h"
 
 namespace t0b {
 
@@ -87,13 +90,35 @@ __device__ __forceinline__ int64_t RowBound(int32_t offset, int64_t entries) {
   return offset < 0 ? 0 : offset < entries ? offset : entries;
 }
 
-// Streaming multiprocessors of the current device.
+// The current device, and its streaming multiprocessors (asked for once).
+constexpr int kMaxDevices = 64;
+
+inline int CurrentDevice() {
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < kMaxDevices ? device : 0;
+}
+
 inline int RoutedSmCount() {
-  int device = 0, count = 148;
-  if (cudaGetDevice(&device) == cudaSuccess) {
-    cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+  static std::atomic<int> counts[kMaxDevices];
+  const int device = CurrentDevice();
+  int count = counts[device].load(std::memory_order_relaxed);
+  if (count == 0) {
+    if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || count < 1) return 148;
+    counts[device].store(count, std::memory_order_relaxed);
   }
   return count;
+}
+
+// Lets kernel `kKernel` use `bytes` of dynamic shared memory on the current
+// device; asked for once per device and size, since the call costs as much as
+// a launch's share of a small operator.
+template <auto kKernel>
+void AllowShared(int bytes) {
+  static std::atomic<int> allowed[kMaxDevices];
+  const int device = CurrentDevice();
+  if (bytes <= 48 * 1024 || allowed[device].load(std::memory_order_relaxed) >= bytes) return;
+  Check(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "kernel shared memory");
+  allowed[device].store(bytes, std::memory_order_relaxed);
 }
 
 }  // namespace t0b

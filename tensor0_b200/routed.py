@@ -60,18 +60,20 @@ class Int4Weights(NamedTuple):
     group: int
 
 
-def _device(*tensors: torch.Tensor) -> torch.device:
-    device = tensors[0].device
+def _device(*tensors: torch.Tensor) -> int:
+    """Index of the CUDA device that holds all the tensors."""
+    index = tensors[0].get_device()
     for tensor in tensors:
-        if not tensor.is_cuda:
+        other = tensor.get_device()   # -1 for host storage
+        if other < 0 or not tensor.is_cuda:
             raise ValueError("routed storage must be a CUDA tensor (there is no CPU fallback)")
-        if tensor.device != device:
+        if other != index:
             raise ValueError("routed operands must be on one device")
-    return device
+    return index
 
 
 def _packed(tensor: torch.Tensor, shape: tuple, dtype: torch.dtype, what: str) -> int:
-    if tensor.dtype != dtype or tensor.shape != shape or not tensor.is_contiguous():
+    if tensor.dtype is not dtype or tensor.shape != shape or not tensor.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {list(shape)}, got {tensor.dtype} "
                          f"{list(tensor.shape)} with strides {list(tensor.stride())}")
     return tensor.data_ptr()
@@ -79,10 +81,11 @@ def _packed(tensor: torch.Tensor, shape: tuple, dtype: torch.dtype, what: str) -
 
 def _matrix(tensor: torch.Tensor, what: str) -> int:
     """Row stride of a 2-d tensor whose rows are contiguous."""
-    if tensor.ndim != 2 or (tensor.shape[1] > 1 and tensor.stride(1) != 1):
+    rows, width = tensor.shape
+    stride, step = tensor.stride()
+    if step != 1 and width > 1:
         raise ValueError(f"{what} must be 2-d with contiguous rows")
-    stride = tensor.stride(0)
-    return stride if tensor.shape[0] > 1 else max(stride, tensor.shape[1])
+    return stride if rows > 1 or stride > width else width
 
 
 def _code(table: dict, tensor: torch.Tensor, what: str) -> int:
@@ -92,14 +95,16 @@ def _code(table: dict, tensor: torch.Tensor, what: str) -> int:
     return code
 
 
-def _call(name: str, device: torch.device, *arguments) -> None:
+def _call(name: str, device: int, *arguments) -> None:
     function = getattr(_native.lib(), name)
     err = _native.error_buffer()
-    if torch.cuda.current_device() == device.index:
-        status = function(*arguments, torch.cuda.current_stream(device).cuda_stream, err, len(err))
+    # The stream's handle alone: building a Stream object costs more than the checks.
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch._C._cuda_getDevice() == device:
+        status = function(*arguments, stream, err, len(err))
     else:
         with torch.cuda.device(device):
-            status = function(*arguments, torch.cuda.current_stream(device).cuda_stream, err, len(err))
+            status = function(*arguments, stream, err, len(err))
     if status != 0:
         _native.check(status, err)
 
@@ -110,9 +115,9 @@ def _entries(routing: Routing) -> tuple[int, int, int]:
         raise ValueError("routing experts must be [tokens, top_k]")
     tokens, top_k = routing.experts.shape
     _packed(routing.rows, (tokens * top_k,), torch.int32, "routing rows")
-    if routing.offsets.ndim != 1 or routing.offsets.numel() < 2:
-        raise ValueError("routing offsets must be [experts + 1]")
     experts = routing.offsets.numel() - 1
+    if experts < 1:
+        raise ValueError("routing offsets must be [experts + 1]")
     _packed(routing.offsets, (experts + 1,), torch.int32, "routing offsets")
     return tokens, top_k, experts
 
@@ -147,13 +152,12 @@ def route(logits: torch.Tensor, top_k: int, *, groups: int = 1, top_groups: int 
     if logits.ndim != 2:
         raise ValueError("logits must be [tokens, experts]")
     tokens, experts = logits.shape
-    given = [t for t in (bias, mask) if t is not None]
-    device = _device(logits, *given)
+    device = _device(logits, *(t for t in (bias, mask) if t is not None))
     code = _code(_FLOAT, logits, "logits")
     bias_pointer = None if bias is None else _packed(bias, (experts,), torch.float32, "bias")
     mask_pointer = None if mask is None else _packed(mask, (tokens,), torch.bool, "mask")
     if out is None:
-        out = empty_routing(tokens, top_k, experts, device)
+        out = empty_routing(tokens, top_k, experts, logits.device)
     else:
         _device(logits, *out)
     entry = (tokens, top_k)
@@ -163,7 +167,7 @@ def route(logits: torch.Tensor, top_k: int, *, groups: int = 1, top_groups: int 
                 _packed(out.positions, entry, torch.int32, "routing positions"),
                 _packed(out.offsets, (experts + 1,), torch.int32, "routing offsets"))
     size = _native.lib().t0b_route_workspace(tokens, experts)
-    workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    workspace = logits.new_empty(size, dtype=torch.uint8) if size else None
     _call("t0b_route", device, code, tokens, experts, top_k, groups, groups if top_groups is None else top_groups,
           group_best, _score(score), int(renormalize), scale, logits.data_ptr(), _matrix(logits, "logits"),
           bias_pointer, mask_pointer, *pointers, None if workspace is None else workspace.data_ptr(), size)
@@ -186,7 +190,7 @@ def route_backward(logits: torch.Tensor, routing: Routing, weights_grad: torch.T
     chosen = _packed(routing.experts, (tokens, top_k), torch.int32, "routing experts")
     grad = _packed(weights_grad, (tokens, top_k), torch.float32, "weights_grad")
     if out is None:
-        out = torch.empty((tokens, experts), dtype=logits.dtype, device=device)
+        out = logits.new_empty((tokens, experts))
     result = _packed(out, (tokens, experts), logits.dtype, "out")
     _call("t0b_route_backward", device, code, tokens, experts, top_k, _score(score), int(renormalize), scale,
           logits.data_ptr(), _matrix(logits, "logits"), chosen, grad, result)
@@ -217,7 +221,7 @@ def routed_matmul(x: torch.Tensor, w: torch.Tensor, routing: Routing, *, gather:
     _operand(x, outer if transpose else inner, gather, tokens, top_k, "x")
     width = inner if transpose else outer
     if out is None:
-        out = torch.empty((tokens * top_k, width), dtype=x.dtype, device=device)
+        out = x.new_empty((tokens * top_k, width))
     else:
         _device(x, out)
     result = _packed(out, (tokens * top_k, width), x.dtype, "out")
@@ -243,7 +247,7 @@ def routed_weight_grad(x: torch.Tensor, y_grad: torch.Tensor, routing: Routing, 
     _operand(x, inner, gather_x, tokens, top_k, "x")
     _operand(y_grad, outer, gather_y, tokens, top_k, "y_grad")
     if out is None:
-        out = torch.empty((experts, inner, outer), dtype=x.dtype, device=device)
+        out = x.new_empty((experts, inner, outer))
     else:
         _device(x, out)
     result = _packed(out, (experts, inner, outer), x.dtype, "out")
@@ -265,7 +269,7 @@ def routed_sum(y: torch.Tensor, routing: Routing, *, out: torch.Tensor | None = 
         raise ValueError(f"y must be [{tokens * top_k}, width]")
     width = y.shape[1]
     if out is None:
-        out = torch.empty((tokens, width), dtype=y.dtype, device=device)
+        out = y.new_empty((tokens, width))
     else:
         _device(y, out)
     result = _packed(out, (tokens, width), y.dtype, "out")
@@ -300,9 +304,9 @@ def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 
         raise ValueError("checkpoint group must be 32, 64 or 128")
     scales = 2 * -(-width // group)
     if out is None:
-        a = torch.empty((rows, width), dtype=h.dtype, device=device)
-        kept = Checkpoint(torch.empty((rows, 2 * width), dtype=torch.int8, device=device),
-                          torch.empty((rows, scales), dtype=torch.float32, device=device), group)
+        a = h.new_empty((rows, width))
+        kept = Checkpoint(h.new_empty((rows, 2 * width), dtype=torch.int8),
+                          h.new_empty((rows, scales), dtype=torch.float32), group)
     else:
         a, kept = out
         if kept.group != group:
@@ -342,10 +346,9 @@ def gated_backward(checkpoint: Checkpoint, a_grad: torch.Tensor, *, routing: Rou
     if a_grad.shape != (rows, width):
         raise ValueError(f"a_grad must be [{rows}, {width}]")
     weights = _row_weights(routing, rows)
-    h_grad = torch.empty((rows, 2 * width), dtype=a_grad.dtype, device=device)
-    a = torch.empty((rows, width), dtype=a_grad.dtype, device=device)
-    weights_grad = torch.empty((rows,) if routing is None else tuple(routing.weights.shape), dtype=torch.float32,
-                               device=device)
+    h_grad = a_grad.new_empty((rows, 2 * width))
+    a = a_grad.new_empty((rows, width))
+    weights_grad = a_grad.new_empty((rows,) if routing is None else routing.weights.shape, dtype=torch.float32)
     _call("t0b_gated_backward", device, code, rows, width, checkpoint.group, codes, scales, a_grad.data_ptr(),
           _matrix(a_grad, "a_grad"), *weights, h_grad.data_ptr(), a.data_ptr(), weights_grad.data_ptr())
     return h_grad, a, weights_grad
@@ -357,7 +360,7 @@ def checkpoint_load(checkpoint: Checkpoint, dtype: torch.dtype = torch.float32) 
     device = _device(checkpoint.codes, checkpoint.scales)
     if dtype not in _FLOAT:
         raise ValueError("checkpoints load as float32, float16 or bfloat16")
-    values = torch.empty((rows, 2 * width), dtype=dtype, device=device)
+    values = checkpoint.codes.new_empty((rows, 2 * width), dtype=dtype)
     _call("t0b_checkpoint_load", device, _FLOAT[dtype], rows, width, checkpoint.group, codes, scales,
           values.data_ptr())
     return values
@@ -398,7 +401,7 @@ def routed_matvec(x: torch.Tensor, weights: Int4Weights, routing: Routing, *, ga
     scale_pointer = _packed(scales, (experts, outer, inner // group), x.dtype, "4-bit weight scales")
     _operand(x, inner, gather, tokens, top_k, "x")
     if out is None:
-        out = torch.empty((tokens * top_k, outer), dtype=x.dtype, device=device)
+        out = x.new_empty((tokens * top_k, outer))
     else:
         _device(x, out)
     result = _packed(out, (tokens * top_k, outer), x.dtype, "out")
