@@ -10,9 +10,17 @@
 // A logit of -inf or NaN, and a masked token, take no expert (index -1,
 // weight 0).  Under softmax a NaN or +inf logit makes the row's weights NaN.
 //
-// One warp holds a token: expert e is value e / 32 of lane e % 32, so loads
-// coalesce.  A pick is two warp reductions: the largest choice value as an
-// ordered integer, then the lowest index that holds it.
+// One warp holds a token: lane l has the kV experts from l * kV on.  A pick is a
+// warp reduction of the choice values as ordered integers and a ballot: the
+// first lane that holds the largest has the lowest index.  Bound by these
+// instructions, not by memory, so nothing else is done for all experts where it
+// can be done for the chosen ones: without a bias the scores are taken of those
+// alone, and where the weights are renormalised the softmax needs no sum over
+// all experts.
+//
+// The row order takes three launches: experts counted per block of tokens, the
+// counts summed over the blocks before each, entries placed.  Few tokens take
+// one block that does it all.
 #include <algorithm>
 #include <climits>
 
@@ -51,57 +59,123 @@ __device__ __forceinline__ double WarpSum(double v) {
   return v;
 }
 
+// The lane's experts of a token; `vector`: as one access (rows start on
+// multiples of it).
 template <typename T, int V>
-__device__ __forceinline__ void LoadLogits(const T* row, int experts, int lane, float (&x)[V]) {
+__device__ __forceinline__ void LoadLogits(const T* row, int experts, int lane, bool vector, float (&x)[V]) {
+  constexpr int kBytes = V * static_cast<int>(sizeof(T));
+  const int first = lane * V;
+  if (vector && first + V <= experts) {
+    alignas(16) T v[V];
+    if constexpr (kBytes % 16 == 0) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int e = j * 32 + lane;
-    x[j] = e < experts ? ToFloat(row[e]) : -INFINITY;
-  }
-}
-
-// The scores of one token.  The softmax normaliser is summed in 64 bits and
-// rounded once, so that it does not depend on the order of the terms and the
-// choice of experts does not either.
-template <int V>
-__device__ __forceinline__ void Scores(const float (&x)[V], int experts, int lane, bool softmax, float (&s)[V]) {
-  if (softmax) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < V; ++j) top = fmaxf(top, x[j]);
-    top = WarpMax(top);
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      s[j] = j * 32 + lane < experts ? expf(x[j] - top) : 0.0f;
-      sum += static_cast<double>(s[j]);
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(row + first)[i];
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(row + first);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(row + first);
+    } else {
+      v[0] = row[first];
     }
-    const float total = static_cast<float>(WarpSum(sum));
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = __fdiv_rn(s[j], total);
+    for (int j = 0; j < V; ++j) x[j] = ToFloat(v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = __frcp_rn(1.0f + expf(-x[j]));
+    for (int j = 0; j < V; ++j) x[j] = first + j < experts ? ToFloat(row[first + j]) : -INFINITY;
   }
 }
 
-// Value `index` (expert number) of a token's register array, in every lane.
-template <int V>
-__device__ __forceinline__ float Pick(const float (&v)[V], int index) {
-  float mine = 0.0f;
+template <typename T, int V>
+bool VectorLogits(const void* logits, int64_t stride) {
+  constexpr uintptr_t kBytes = V * sizeof(T) < 16 ? V * sizeof(T) : 16;
+  return reinterpret_cast<uintptr_t>(logits) % kBytes == 0 && static_cast<uint64_t>(stride) * sizeof(T) % kBytes == 0;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void StoreValues(T* row, int experts, int lane, bool vector, const float (&d)[V]) {
+  constexpr int kBytes = V * static_cast<int>(sizeof(T));
+  const int first = lane * V;
+  alignas(16) T v[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = FromFloat<T>(d[j]);
+  if (vector && first + V <= experts) {
+    if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(row + first)[i] = reinterpret_cast<const uint4*>(v)[i];
+      return;
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(row + first) = *reinterpret_cast<const uint2*>(v);
+      return;
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(row + first) = *reinterpret_cast<const uint32_t*>(v);
+      return;
+    }
+  }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    if (j == (index >> 5)) mine = v[j];
+    if (first + j < experts) row[first + j] = v[j];
   }
-  return __shfl_sync(kFull, mine, index & 31);
 }
 
-// Chosen experts and weights of the block's tokens.  `choices` is one row of
-// experts per warp (groups only).
-template <typename T, int V>
-__device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, int64_t end, float* choices) {
+// Largest logit of the token; exp(x - largest) is at most 1.
+template <int V>
+__device__ __forceinline__ float Largest(const float (&x)[V]) {
+  float top = x[0];
+#pragma unroll
+  for (int j = 1; j < V; ++j) top = fmaxf(top, x[j]);
+  return WarpMax(top);
+}
+
+// Inverse of Ordered.
+__device__ __forceinline__ float Unordered(uint32_t key) {
+  return __uint_as_float((key >> 31) != 0 ? key ^ 0x80000000u : ~key);
+}
+
+// Of each group of `size` experts the best value, or the sum of its two best;
+// lane g has group g's.  `values`: one row per warp of shared memory.
+template <int V>
+__device__ __forceinline__ float GroupScore(const float (&c)[V], int experts, int groups, int best, float* values) {
+  const int lane = threadIdx.x & 31, size = experts / groups;
+  float first = -INFINITY, second = -INFINITY;
+  const auto add = [&](float v) {
+    second = fmaxf(second, fminf(first, v));
+    first = fmaxf(first, v);
+  };
+  // Lanes per group where a group is a power of two of whole lanes; otherwise
+  // through shared memory, with as many lanes to a group as there are.
+  int lanes = size / V, source;
+  if (size % V == 0 && (lanes & (lanes - 1)) == 0) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) add(c[j]);
+    source = lane * lanes;
+  } else {
+    lanes = 1;
+    while (lanes * 2 * groups <= 32) lanes *= 2;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (lane * V + j < experts) values[lane * V + j] = c[j];
+    }
+    __syncwarp();
+    if (lane / lanes < groups) {
+      for (int i = lane % lanes; i < size; i += lanes) add(values[lane / lanes * size + i]);
+    }
+    source = lane * lanes;
+  }
+  for (int d = 1; d < lanes; d <<= 1) {
+    const float f = __shfl_xor_sync(kFull, first, d), s = __shfl_xor_sync(kFull, second, d);
+    second = fmaxf(fmaxf(second, s), fminf(first, f));
+    first = fmaxf(first, f);
+  }
+  if (best == 2 && second > -INFINITY) first += second;
+  return __shfl_sync(kFull, first, source & 31);
+}
+
+// Chosen experts and weights of the block's tokens.  kByLogit: the choice goes
+// by the logits.
+template <typename T, int V, bool kByLogit>
+__device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, int64_t end, float* values, bool vector) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const bool by_logit = a.bias == nullptr && a.group_best == 1;
   for (int64_t t = begin + warp; t < end; t += warps) {
     int32_t* chosen = a.chosen + t * a.top_k;
     float* weights = a.weights + t * a.top_k;
@@ -112,85 +186,102 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
       }
       continue;
     }
-    float x[V], s[V];
-    LoadLogits<T, V>(static_cast<const T*>(a.logits) + t * a.logit_stride, a.experts, lane, x);
-    Scores<V>(x, a.experts, lane, a.softmax != 0, s);
+    float x[V], c[V];   // c: what the choice goes by
+    LoadLogits<T, V>(static_cast<const T*>(a.logits) + t * a.logit_stride, a.experts, lane, vector, x);
+    float top = 0.0f, total = 1.0f;
+    bool nan = false;
+    if (a.softmax != 0) {
+      top = Largest<V>(x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) nan = nan || x[j] != x[j];
+      nan = __any_sync(kFull, nan);
+    }
+    if constexpr (kByLogit) {
+      if (a.softmax != 0 && (a.renormalize == 0 || a.groups > 1)) {
+        // With renormalised weights and one group the sum would cancel: the
+        // chosen scores hold at least 1 / experts of it, beside which 1e-20 is nothing.
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += lane * V + j < a.experts ? expf(x[j] - top) : 0.0f;
+        total = WarpSum(sum);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) c[j] = x[j];
+    } else {
+      if (a.softmax != 0) {
+        // Summed in 64 bits and rounded once: the choice, which goes by these
+        // scores, does not depend on the order of the terms.
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          c[j] = lane * V + j < a.experts ? expf(x[j] - top) : 0.0f;
+          sum += static_cast<double>(c[j]);
+        }
+        total = static_cast<float>(WarpSum(sum));
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] = __fdiv_rn(c[j], total);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] = __frcp_rn(1.0f + expf(-x[j]));
+      }
+      if (a.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) c[j] += lane * V + j < a.experts ? a.bias[lane * V + j] : 0.0f;
+      }
+    }
     uint32_t key[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int e = j * 32 + lane;
-      float c = by_logit ? x[j] : s[j];
-      if (a.bias != nullptr && e < a.experts) c += a.bias[e];
-      key[j] = x[j] > -INFINITY && c > -INFINITY ? Ordered(c) : 0u;
-      if (a.groups > 1 && e < a.experts) {
-        choices[warp * a.experts + e] = key[j] != 0u ? c : -INFINITY;
-      }
+      const bool some = x[j] > -INFINITY && c[j] > -INFINITY;
+      key[j] = some ? Ordered(c[j]) : 0u;
+      if (!some) c[j] = -INFINITY;
     }
     if (a.groups > 1) {
-      __syncwarp();
-      const int size = a.experts / a.groups;
-      uint32_t group_key = 0;
-      if (lane < a.groups) {
-        float first = -INFINITY, second = -INFINITY;
-        const float* mine = choices + warp * a.experts + lane * size;
-        // Lanes start at different places of their groups, which spreads the banks.
-        int i = lane % size;
-        for (int n = 0; n < size; ++n) {
-          const float c = mine[i];
-          second = fmaxf(second, fminf(first, c));
-          first = fmaxf(first, c);
-          if (++i == size) i = 0;
-        }
-        if (a.group_best == 2 && second > -INFINITY) first += second;
-        group_key = Ordered(first);
-      }
-      __syncwarp();
-      uint32_t kept = 0;
+      const float score = GroupScore<V>(c, a.experts, a.groups, a.group_best, values + warp * a.experts);
+      uint32_t group_key = lane < a.groups ? Ordered(score) : 0u, kept = 0;
       for (int n = 0; n < a.top_groups; ++n) {
         const uint32_t best = __reduce_max_sync(kFull, group_key);
-        const uint32_t holders = __ballot_sync(kFull, group_key == best && lane < a.groups);
-        const int winner = __ffs(holders) - 1;
-        if (winner < 0) break;
+        const int winner = __ffs(__ballot_sync(kFull, group_key == best)) - 1;
         kept |= 1u << winner;
-        if (lane == winner) group_key = 0;
+        if (lane == winner) group_key = 0u;
       }
+      const int size = a.experts / a.groups;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int e = j * 32 + lane;
+        const int e = lane * V + j;
         if (e < a.experts && ((kept >> (e / size)) & 1u) == 0u) key[j] = 0u;
       }
     }
     int mine = -1;
-    float score = 0.0f;
+    uint32_t mine_key = 0;
     for (int n = 0; n < a.top_k; ++n) {
-      uint32_t best = 0;
-      int at = 0;
-      float value = 0.0f;
+      uint32_t best = key[0];
+#pragma unroll
+      for (int j = 1; j < V; ++j) best = max(best, key[j]);
+      const uint32_t largest = __reduce_max_sync(kFull, best);
+      if (largest == 0u) break;
+      const int winner = __ffs(__ballot_sync(kFull, best == largest)) - 1;
+      int at = V - 1;
+#pragma unroll
+      for (int j = V - 2; j >= 0; --j) at = key[j] == largest ? j : at;
+      const int index = __shfl_sync(kFull, lane * V + at, winner);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (key[j] > best) {
-          best = key[j];
-          at = j;
-          value = s[j];
-        }
+        if (lane * V + j == index) key[j] = 0u;
       }
-      const uint32_t top = __reduce_max_sync(kFull, best);
-      if (top == 0u) break;
-      const unsigned index = __reduce_min_sync(kFull, best == top ? static_cast<unsigned>(at * 32 + lane) : UINT_MAX);
-      value = __shfl_sync(kFull, value, index & 31);
       if (lane == n) {
-        mine = static_cast<int>(index);
-        score = value;
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (static_cast<unsigned>(j * 32 + lane) == index) key[j] = 0u;
+        mine = index;
+        mine_key = largest;
       }
     }
-    if (a.renormalize != 0) {
-      const float total = WarpSum(score) + 1e-20f;
-      score = __fdiv_rn(score, total);
+    float score = 0.0f;
+    if (mine >= 0) {
+      const float logit = kByLogit ? Unordered(mine_key)
+                                   : ToFloat(static_cast<const T*>(a.logits)[t * a.logit_stride + mine]);
+      score = a.softmax != 0 ? __fdiv_rn(expf(logit - top), total) : __frcp_rn(1.0f + expf(-logit));
+      if (nan) score = __uint_as_float(0x7fc00000u);
     }
+    if (a.renormalize != 0) score = __fdiv_rn(score, WarpSum(score) + 1e-20f);
     if (lane < a.top_k) {
       chosen[lane] = mine;
       weights[lane] = mine < 0 ? 0.0f : score * a.scale;
@@ -274,14 +365,14 @@ __device__ __forceinline__ void CountEntries(const RouteArgs& a, int64_t begin, 
 }
 
 // One block does all: few tokens, where launches cost more than the work.
-template <typename T, int V>
-__global__ void __launch_bounds__(1024) RouteOneBlock(RouteArgs a) {
+template <typename T, int V, bool kByLogit>
+__global__ void __launch_bounds__(1024) RouteOneBlock(RouteArgs a, bool vector) {
   extern __shared__ int route_smem[];
   int* first = route_smem;                        // experts + 1
   int* by_warp = first + a.experts + 1;           // warps x (experts + 1)
-  float* choices = reinterpret_cast<float*>(by_warp);   // reused: the choice is over before rows are placed
+  float* values = reinterpret_cast<float*>(by_warp);   // reused: the choice is over before rows are placed
   for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) first[e] = 0;
-  SelectTokens<T, V>(a, 0, a.tokens, choices);
+  SelectTokens<T, V, kByLogit>(a, 0, a.tokens, values, vector);
   __syncthreads();
   CountEntries(a, 0, a.tokens * a.top_k, first);
   __syncthreads();
@@ -291,63 +382,94 @@ __global__ void __launch_bounds__(1024) RouteOneBlock(RouteArgs a) {
   PlaceEntries(a, 0, a.tokens * a.top_k, first, by_warp);
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(kRouteThreads) RouteSelect(RouteArgs a, int64_t tokens_per_block) {
+// The three launches overlap: each starts while the one before it ends, and
+// waits for its writes here.
+__device__ __forceinline__ void LetNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void WaitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename T, int V, bool kByLogit>
+__global__ void __launch_bounds__(kRouteThreads) RouteSelect(RouteArgs a, int64_t tokens_per_block, bool vector) {
   extern __shared__ int route_smem[];
+  LetNextStart();
   int* bins = route_smem;
-  float* choices = reinterpret_cast<float*>(bins + a.experts);
+  float* values = reinterpret_cast<float*>(bins + a.experts);
   for (int e = threadIdx.x; e < a.experts; e += blockDim.x) bins[e] = 0;
   const int64_t begin = blockIdx.x * tokens_per_block;
   const int64_t end = begin + tokens_per_block < a.tokens ? begin + tokens_per_block : a.tokens;
-  SelectTokens<T, V>(a, begin, end, choices);
+  SelectTokens<T, V, kByLogit>(a, begin, end, values, vector);
   __syncthreads();
   CountEntries(a, begin * a.top_k, end * a.top_k, bins);
   __syncthreads();
   for (int e = threadIdx.x; e < a.experts; e += blockDim.x) a.counts[blockIdx.x * int64_t{a.experts} + e] = bins[e];
 }
 
-__global__ void __launch_bounds__(kRouteThreads) RoutePlace(RouteArgs a, int64_t tokens_per_block) {
-  extern __shared__ int route_smem[];
-  int* total = route_smem;                  // experts + 1
-  int* before = total + a.experts + 1;      // experts + 1
-  int* by_warp = before + a.experts + 1;
-  for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) total[e] = before[e] = 0;
-  __syncthreads();
-  // Threads share the blocks' counts: several of them sum one expert's column.
-  const int lanes = a.experts < static_cast<int>(blockDim.x) ? a.experts : static_cast<int>(blockDim.x);
-  const int parts = static_cast<int>(blockDim.x) / lanes;
-  const int part = static_cast<int>(threadIdx.x) / lanes;
-  if (part < parts) {
-    for (int e = static_cast<int>(threadIdx.x) % lanes; e < a.experts; e += lanes) {
-      int all = 0, mine = 0;
+// Each block's counts become the counts of the blocks before it; the totals go
+// in the row after the last block's.  A block has 32 experts, a warp a run of
+// the counting blocks.
+constexpr int kScanWarps = 32;
+__global__ void __launch_bounds__(kScanWarps * 32) RouteScan(RouteArgs a, int blocks) {
+  __shared__ int sums[kScanWarps][33];
+  LetNextStart();
+  WaitForPrevious();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+  const int run = (blocks + kScanWarps - 1) / kScanWarps, from = warp * run, to = min(blocks, from + run);
+  int sum = 0;
+  if (e < a.experts) {
 #pragma unroll 8
-      for (unsigned b = static_cast<unsigned>(part); b < gridDim.x; b += static_cast<unsigned>(parts)) {
-        const int count = a.counts[b * int64_t{a.experts} + e];
-        all += count;
-        mine += b < blockIdx.x ? count : 0;
-      }
-      atomicAdd(total + e, all);
-      atomicAdd(before + e, mine);
-    }
+    for (int b = from; b < to; ++b) sum += a.counts[b * int64_t{a.experts} + e];
   }
+  sums[warp][lane] = sum;
   __syncthreads();
-  PrefixByWarp(total, a.experts);
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    int present = 0;
-    for (int e = threadIdx.x; e < a.experts; e += 32) present += before[e];
-    present = __reduce_add_sync(kFull, present);
-    if (threadIdx.x == 0) before[a.experts] = static_cast<int>(blockIdx.x * tokens_per_block * a.top_k) - present;
+  if (e >= a.experts) return;
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kScanWarps; ++w) {
+    before += w < warp ? sums[w][lane] : 0;
+    all += sums[w][lane];
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e <= a.experts; e += blockDim.x) {
-    if (blockIdx.x == 0) a.offsets[e] = total[e];
-    before[e] += total[e];
+#pragma unroll 8
+  for (int b = from; b < to; ++b) {
+    int32_t* cell = a.counts + b * int64_t{a.experts} + e;
+    const int count = *cell;
+    *cell = before;
+    before += count;
   }
+  if (warp == 0) a.counts[blocks * int64_t{a.experts} + e] = all;
+}
+
+constexpr int kPlaceThreads = 128;
+__global__ void __launch_bounds__(kPlaceThreads) RoutePlace(RouteArgs a, int64_t tokens_per_block) {
+  extern __shared__ int route_smem[];
+  int* first = route_smem;                  // experts + 1
+  int* by_warp = first + a.experts + 1;
+  WaitForPrevious();
+  const int32_t* totals = a.counts + gridDim.x * int64_t{a.experts};
+  for (int e = threadIdx.x; e < a.experts; e += kPlaceThreads) first[e] = totals[e];
+  __syncthreads();
+  PrefixByWarp(first, a.experts);
   __syncthreads();
   const int64_t begin = blockIdx.x * tokens_per_block;
   const int64_t end = begin + tokens_per_block < a.tokens ? begin + tokens_per_block : a.tokens;
-  PlaceEntries(a, begin * a.top_k, end * a.top_k, before, by_warp);
+  int present = 0;   // entries with an expert before this block
+  for (int e = threadIdx.x; e <= a.experts; e += kPlaceThreads) {
+    if (blockIdx.x == 0) a.offsets[e] = first[e];
+    if (e < a.experts) {
+      const int before = a.counts[blockIdx.x * int64_t{a.experts} + e];
+      present += before;
+      first[e] += before;
+    }
+  }
+  present = __reduce_add_sync(kFull, present);
+  int* absent = first + a.experts;   // holds the entries that have an expert
+  if ((threadIdx.x & 31) == 0) by_warp[threadIdx.x >> 5] = present;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int sum = 0;
+    for (int w = 0; w < kPlaceThreads / 32; ++w) sum += by_warp[w];
+    *absent += static_cast<int>(begin * a.top_k) - sum;
+  }
+  __syncthreads();
+  PlaceEntries(a, begin * a.top_k, end * a.top_k, first, by_warp);
 }
 
 // With g = scale * (gradient of the chosen weights) and p the chosen scores:
@@ -356,90 +478,123 @@ __global__ void __launch_bounds__(kRouteThreads) RoutePlace(RouteArgs a, int64_t
 //   sigmoid: dx_j = ds_j s_j (1 - s_j)
 // Memory bound: reads and writes each logit once; the scores are recomputed.
 template <typename T, int V>
-__global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs a) {
+__global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs a, bool vector) {
+  extern __shared__ float scattered[];   // one row of experts per warp: ds, zero between tokens
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int64_t step = int64_t{gridDim.x} * warps;
+  float* ds = scattered + warp * (32 * V);
+#pragma unroll
+  for (int j = 0; j < V; ++j) ds[j * 32 + lane] = 0.0f;
+  __syncwarp();
   for (int64_t t = int64_t{blockIdx.x} * warps + warp; t < a.tokens; t += step) {
     T* out = static_cast<T*>(a.logits_grad) + t * a.experts;
+    const T* row = static_cast<const T*>(a.logits) + t * a.logit_stride;
     const int mine = lane < a.top_k ? a.chosen[t * a.top_k + lane] : -1;
-    float g = mine >= 0 ? a.weights_grad[t * a.top_k + lane] * a.scale : 0.0f;
-    if (__ballot_sync(kFull, mine >= 0) == 0u) {   // no expert: the logits may hold anything
+    const bool found = mine >= 0 && mine < a.experts;
+    float g = found ? a.weights_grad[t * a.top_k + lane] * a.scale : 0.0f;
+    float d[V];
+    if (__ballot_sync(kFull, found) == 0u) {   // no expert: the logits may hold anything
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (j * 32 + lane < a.experts) out[j * 32 + lane] = FromFloat<T>(0.0f);
+      for (int j = 0; j < V; ++j) d[j] = 0.0f;
+    } else {
+      float x[V], top = 0.0f, inverse = 1.0f, p = 0.0f;
+      LoadLogits<T, V>(row, a.experts, lane, vector, x);
+      const float logit = found ? ToFloat(row[mine]) : 0.0f;
+      if (a.softmax != 0) {
+        top = Largest<V>(x);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          x[j] = lane * V + j < a.experts ? expf(x[j] - top) : 0.0f;
+          sum += x[j];
+        }
+        inverse = __frcp_rn(WarpSum(sum));
+        if (found) p = expf(logit - top) * inverse;
+      } else if (found) {
+        p = __frcp_rn(1.0f + expf(-logit));
       }
-      continue;
-    }
-    float x[V], s[V], ds[V];
-    LoadLogits<T, V>(static_cast<const T*>(a.logits) + t * a.logit_stride, a.experts, lane, x);
-    Scores<V>(x, a.experts, lane, a.softmax != 0, s);
-    float p = 0.0f;
-    for (int n = 0; n < a.top_k; ++n) {
-      const int index = __shfl_sync(kFull, mine, n);
-      const float value = Pick<V>(s, index < 0 ? 0 : index);
-      if (lane == n && index >= 0) p = value;
-    }
-    if (a.renormalize != 0) {
-      const float total = WarpSum(p) + 1e-20f;
-      const float mean = WarpSum(g * __fdiv_rn(p, total));
-      g = mine >= 0 ? __fdiv_rn(g - mean, total) : 0.0f;
-    }
-    const float inner = WarpSum(g * p);
-#pragma unroll
-    for (int j = 0; j < V; ++j) ds[j] = 0.0f;
-    for (int n = 0; n < a.top_k; ++n) {
-      const int index = __shfl_sync(kFull, mine, n);
-      const float value = __shfl_sync(kFull, g, n);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (j * 32 + lane == index) ds[j] = value;
+      if (a.renormalize != 0) {
+        const float total = __frcp_rn(WarpSum(p) + 1e-20f);
+        const float mean = WarpSum(g * (p * total));
+        g = found ? (g - mean) * total : 0.0f;
       }
-    }
+      if (found) ds[mine] = g;
+      __syncwarp();
+      if (a.softmax != 0) {
+        const float inner = WarpSum(g * p);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = j * 32 + lane;
-      if (e >= a.experts) continue;
-      const float d = a.softmax != 0 ? s[j] * (ds[j] - inner) : ds[j] * s[j] * (1.0f - s[j]);
-      out[e] = FromFloat<T>(d);
+        for (int j = 0; j < V; ++j) d[j] = x[j] * inverse * (ds[lane * V + j] - inner);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float g_j = ds[lane * V + j];
+          const float s = __frcp_rn(1.0f + expf(-x[j]));
+          d[j] = g_j != 0.0f ? g_j * s * (1.0f - s) : 0.0f;
+        }
+      }
+      __syncwarp();
+      if (found) ds[mine] = 0.0f;
+      __syncwarp();
     }
+    StoreValues<T, V>(out, a.experts, lane, vector, d);
   }
 }
 
 // Up to this many tokens one block does the whole call.
 constexpr int64_t kOneBlockTokens = 64;
 
+// Counting blocks: enough to fill the device with warps, each with its eight
+// warps' tokens at least.
 int64_t TokensPerBlock(int64_t tokens) {
-  const int64_t blocks = int64_t{RoutedSmCount()} * 2;
-  return std::max<int64_t>(8, (tokens + blocks - 1) / blocks);
+  const int64_t blocks = int64_t{RoutedSmCount()} * 4;
+  return std::max<int64_t>(8, ((tokens + blocks - 1) / blocks + 7) / 8 * 8);
 }
 
-template <typename T, int V>
+template <typename... Args>
+void LaunchAfter(void (*kernel)(Args...), unsigned blocks, unsigned threads, std::size_t smem, cudaStream_t stream,
+                 Args... args) {
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(blocks);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &overlap;
+  config.numAttrs = 1;
+  Check(cudaLaunchKernelEx(&config, kernel, args...), "row order launch");
+}
+
+template <typename T, int V, bool kByLogit>
 void Route(const RouteArgs& a, cudaStream_t stream) {
   const std::size_t bins = static_cast<std::size_t>(a.experts) + 1;
+  const bool vector = VectorLogits<T, V>(a.logits, a.logit_stride);
   if (a.tokens <= kOneBlockTokens) {
     const unsigned warps = static_cast<unsigned>(std::min<int64_t>(32, std::max<int64_t>(1, a.tokens)));
     const std::size_t smem = (bins + warps * bins) * sizeof(int);
-    AllowShared<RouteOneBlock<T, V>>(static_cast<int>(smem));
-    RouteOneBlock<T, V><<<1, warps * 32, smem, stream>>>(a);
+    AllowShared<RouteOneBlock<T, V, kByLogit>>(static_cast<int>(smem));
+    RouteOneBlock<T, V, kByLogit><<<1, warps * 32, smem, stream>>>(a, vector);
     Check(cudaGetLastError(), "router launch");
     g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
     return;
   }
   const int64_t per_block = TokensPerBlock(a.tokens);
   const unsigned blocks = static_cast<unsigned>((a.tokens + per_block - 1) / per_block);
-  const int warps = kRouteThreads / 32;
-  const std::size_t select = (bins + (a.groups > 1 ? warps * bins : 0)) * sizeof(int);
-  RouteSelect<T, V><<<blocks, kRouteThreads, select, stream>>>(a, per_block);
+  const std::size_t select = (bins + (a.groups > 1 ? kRouteThreads / 32 * bins : 0)) * sizeof(int);
+  RouteSelect<T, V, kByLogit><<<blocks, kRouteThreads, select, stream>>>(a, per_block, vector);
   Check(cudaGetLastError(), "router launch");
-  RoutePlace<<<blocks, kRouteThreads, (2 + warps) * bins * sizeof(int), stream>>>(a, per_block);
-  Check(cudaGetLastError(), "row order launch");
-  g_kernel_launches.fetch_add(2, std::memory_order_relaxed);
+  LaunchAfter(RouteScan, static_cast<unsigned>((a.experts + 31) / 32), kScanWarps * 32, 0, stream, a,
+              static_cast<int>(blocks));
+  LaunchAfter(RoutePlace, blocks, kPlaceThreads, (1 + kPlaceThreads / 32) * bins * sizeof(int), stream, a, per_block);
+  g_kernel_launches.fetch_add(3, std::memory_order_relaxed);
 }
 
 template <typename T, int V>
 void Backward(const RouteBackwardArgs& a, cudaStream_t stream) {
   const int64_t blocks = std::min<int64_t>((a.tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32), 1 << 20);
-  RouteBackward<T, V><<<static_cast<unsigned>(blocks), kRouteThreads, 0, stream>>>(a);
+  const bool vector = VectorLogits<T, V>(a.logits, a.logit_stride) && VectorLogits<T, V>(a.logits_grad, a.experts);
+  RouteBackward<T, V><<<static_cast<unsigned>(blocks), kRouteThreads, kRouteThreads * V * sizeof(float), stream>>>(a, vector);
   Check(cudaGetLastError(), "router gradient launch");
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
 }
@@ -468,13 +623,18 @@ void ByType(int32_t dtype, Body&& body) {
 std::size_t RouteWorkspace(int64_t tokens, int experts) {
   if (tokens <= kOneBlockTokens) return 0;
   const int64_t per_block = TokensPerBlock(tokens);
-  return static_cast<std::size_t>((tokens + per_block - 1) / per_block) * experts * sizeof(int32_t);
+  // A row of counts per block, and their totals.
+  return static_cast<std::size_t>((tokens + per_block - 1) / per_block + 1) * experts * sizeof(int32_t);
 }
 
 void LaunchRoute(int32_t dtype, const RouteArgs& args, cudaStream_t stream) {
   ByType(dtype, [&](auto type) {
     using T = decltype(type);
-    ByExperts<T>(args, [&](auto values) { Route<T, decltype(values)::value>(args, stream); });
+    ByExperts<T>(args, [&](auto values) {
+      constexpr int V = decltype(values)::value;
+      if (args.bias == nullptr && args.group_best == 1) Route<T, V, true>(args, stream);
+      else Route<T, V, false>(args, stream);
+    });
   });
 }
 

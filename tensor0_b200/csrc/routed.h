@@ -30,7 +30,7 @@ struct RouteArgs {
   int32_t* rows;           // [tokens * top_k]
   int32_t* positions;      // [tokens, top_k]
   int32_t* offsets;        // [experts + 1]
-  int32_t* counts;         // workspace [blocks, experts]
+  int32_t* counts;         // workspace [counting blocks + 1, experts]
 };
 
 struct RouteBackwardArgs {
