@@ -37,6 +37,61 @@ __device__ __forceinline__ bool RowWeight(const GatedArgs& a, int64_t p, float* 
   return true;
 }
 
+// Eight neighbours as they lie in memory, fetched ahead of their use.
+template <typename T, bool Vector>
+struct Raw8 {
+  uint4 bits;
+  __device__ __forceinline__ void Fetch(const T* p, int count) {
+    bits = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (Vector) {
+      if (count > 0) bits = __ldcs(reinterpret_cast<const uint4*>(p));
+    } else {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = i < count ? reinterpret_cast<const uint16_t*>(p)[i] : 0u;
+      bits = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
+  }
+  __device__ __forceinline__ void Values(float (&v)[8]) const {
+    const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Unpack2<T>(w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+
+template <bool Vector>
+struct RawCodes {
+  uint2 bits;
+  float unit;
+  __device__ __forceinline__ void Fetch(const int8_t* codes, const float* scale, int count) {
+    bits = make_uint2(0u, 0u);
+    unit = 0.0f;
+    if (count <= 0) return;
+    unit = *scale;
+    if constexpr (Vector) {
+      bits = __ldcs(reinterpret_cast<const uint2*>(codes));
+    } else {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = i < count ? static_cast<uint8_t>(codes[i]) : 0u;
+      bits = make_uint2(w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24);
+    }
+  }
+  // A byte c + 128 in the low bits of 2^23 is 2^23 + 128 + c: exact, without a conversion.
+  __device__ __forceinline__ void Values(float (&v)[8]) const {
+    const uint32_t biased[2] = {bits.x ^ 0x80808080u, bits.y ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t word = __byte_perm(biased[i >> 2], 0x4b000000u, 0x7650 | (i & 3));
+      v[i] = (__uint_as_float(word) - 8388736.0f) * unit;
+    }
+  }
+};
+
 // Codes of eight values and, by the group's first lane, the group's scale.
 // A NaN's magnitude bits are above infinity's, so the integer maximum keeps it.
 template <bool Vector>
@@ -51,102 +106,111 @@ __device__ __forceinline__ void StoreCodes(const float (&v)[8], int count, int l
   const float per_unit = none ? 0.0f : __frcp_rn(largest) * 127.0f;
   if (count <= 0) return;
   if ((lane & (lanes - 1)) == 0) *scale = none ? 0.0f : largest * (1.0f / 127.0f);
-  int q[8];
+  // |v * per_unit| is at most 127 and two roundings, so adding 1.5 * 2^23 rounds
+  // it to a whole number, half to even, in the low byte (a group that is not
+  // finite loads as NaN whatever its codes are).
+  uint32_t q[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = max(-127, min(127, __float2int_rn(v[i] * per_unit)));
+  for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], per_unit), 12582912.0f));
   if constexpr (Vector) {
     uint2 packed;
-    packed.x = (q[0] & 255) | ((q[1] & 255) << 8) | ((q[2] & 255) << 16) | (q[3] << 24);
-    packed.y = (q[4] & 255) | ((q[5] & 255) << 8) | ((q[6] & 255) << 16) | (q[7] << 24);
-    *reinterpret_cast<uint2*>(codes) = packed;
+    packed.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    packed.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+    __stcs(reinterpret_cast<uint2*>(codes), packed);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i < count) codes[i] = static_cast<int8_t>(q[i]);
+      if (i < count) codes[i] = static_cast<int8_t>(q[i] & 255u);
     }
   }
 }
 
-template <bool Vector>
-__device__ __forceinline__ void LoadCodes(const int8_t* codes, const float* scale, int count, float (&v)[8]) {
-  if (count <= 0) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    return;
-  }
-  const float unit = *scale;
-  if constexpr (Vector) {
-    const uint2 packed = *reinterpret_cast<const uint2*>(codes);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t word = i < 4 ? packed.x : packed.y;
-      v[i] = static_cast<float>(static_cast<int8_t>(word >> (8 * (i & 3)))) * unit;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? static_cast<float>(codes[i]) * unit : 0.0f;
-  }
-}
-
-// A warp takes 256 columns of one row, of both halves.
+// The columns of a row that a warp takes: 256 at a time, every `parts`-th.
+// blockIdx.y is the part: few rows are split over their columns.
 template <typename T, bool Vector>
-__global__ void __launch_bounds__(kGatedThreads) GatedSave(GatedArgs a, int64_t chunks) {
-  const int lane = threadIdx.x & 31, lanes = a.group / 8;
-  const int groups = (a.width + a.group - 1) / a.group;
-  const int64_t units = a.rows_count * chunks, step = int64_t{gridDim.x} * (kGatedThreads / 32);
-  for (int64_t unit = int64_t{blockIdx.x} * (kGatedThreads / 32) + (threadIdx.x >> 5); unit < units; unit += step) {
-    const int64_t p = unit / chunks;
-    const int column = static_cast<int>(unit - p * chunks) * 256 + lane * 8;
-    const int count = a.width - column;
+__global__ void __launch_bounds__(kGatedThreads) GatedSave(GatedArgs a) {
+  const int lane = threadIdx.x & 31, lanes = a.group / 8, shift = 31 - __clz(a.group);
+  const int groups = (a.width + a.group - 1) >> shift, stride = static_cast<int>(gridDim.y) * 256;
+  const int64_t step = int64_t{gridDim.x} * (kGatedThreads / 32);
+  for (int64_t p = int64_t{blockIdx.x} * (kGatedThreads / 32) + (threadIdx.x >> 5); p < a.rows_count; p += step) {
     float weight;
     int64_t entry;
     const bool present = RowWeight(a, p, &weight, &entry);
-    const T* row = static_cast<const T*>(a.h) + p * a.h_stride + column;
-    float g[8], u[8], out[8];
-    Load8<T, Vector>(row, present ? count : 0, g);
-    Load8<T, Vector>(row + a.width, present ? count : 0, u);
+    const T* row = static_cast<const T*>(a.h) + p * a.h_stride;
+    T* out_row = static_cast<T*>(a.a) + p * a.width;
+    int8_t* code_row = a.codes + p * 2 * a.width;
+    float* scale_row = a.scales + p * 2 * groups;
+    const int begin = static_cast<int>(blockIdx.y) * 256;
+    Raw8<T, Vector> next_g, next_u;
+    const auto fetch = [&](int base) {
+      const int column = base + lane * 8, count = present ? a.width - column : 0;
+      next_g.Fetch(row + column, count);
+      next_u.Fetch(row + a.width + column, count);
+    };
+    fetch(begin);
+    for (int base = begin; base < a.width; base += stride) {
+      const int column = base + lane * 8, count = a.width - column;
+      float g[8], u[8], out[8];
+      next_g.Values(g);
+      next_u.Values(u);
+      if (base + stride < a.width) fetch(base + stride);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = present ? weight * (g[i] * Sigmoid(g[i])) * u[i] : 0.0f;
-    Store8<T, Vector>(static_cast<T*>(a.a) + p * a.width + column, count, out);
-    int8_t* codes = a.codes + p * 2 * a.width + column;
-    float* scales = a.scales + p * 2 * groups + column / a.group;
-    StoreCodes<Vector>(g, count, lanes, lane, codes, scales);
-    StoreCodes<Vector>(u, count, lanes, lane, codes + a.width, scales + groups);
+      for (int i = 0; i < 8; ++i) out[i] = weight * (g[i] * Sigmoid(g[i])) * u[i];
+      if (!present) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] = 0.0f;
+      }
+      Store8<T, Vector>(out_row + column, count, out);
+      StoreCodes<Vector>(g, count, lanes, lane, code_row + column, scale_row + (column >> shift));
+      StoreCodes<Vector>(u, count, lanes, lane, code_row + a.width + column, scale_row + groups + (column >> shift));
+    }
   }
 }
 
 // A warp takes a row: the routing weight's gradient is the row's sum.
 template <typename T, bool Vector>
 __global__ void __launch_bounds__(kGatedThreads) GatedBackward(GatedArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int groups = (a.width + a.group - 1) / a.group;
+  const int lane = threadIdx.x & 31, shift = 31 - __clz(a.group);
+  const int groups = (a.width + a.group - 1) >> shift;
   const int64_t step = int64_t{gridDim.x} * (kGatedThreads / 32);
   for (int64_t p = int64_t{blockIdx.x} * (kGatedThreads / 32) + (threadIdx.x >> 5); p < a.rows_count; p += step) {
     float weight;
     int64_t entry;
     const bool present = RowWeight(a, p, &weight, &entry);
+    const int8_t* code_row = a.codes + p * 2 * a.width;
+    const float* scale_row = a.scales + p * 2 * groups;
+    const T* grad_row = static_cast<const T*>(a.a_grad) + p * a.a_grad_stride;
+    T* h_row = static_cast<T*>(a.h_grad) + p * 2 * a.width;
+    T* out_row = static_cast<T*>(a.a) + p * a.width;
+    RawCodes<Vector> next_g, next_u;
+    Raw8<T, Vector> next_da;
+    const auto fetch = [&](int base) {
+      const int column = base + lane * 8, count = present ? a.width - column : 0;
+      next_g.Fetch(code_row + column, scale_row + (column >> shift), count);
+      next_u.Fetch(code_row + a.width + column, scale_row + groups + (column >> shift), count);
+      next_da.Fetch(grad_row + column, count);
+    };
+    fetch(0);
     float dot = 0.0f;
-    for (int column = lane * 8; column < a.width; column += 256) {
-      const int count = a.width - column;
-      const int8_t* codes = a.codes + p * 2 * a.width + column;
-      const float* scales = a.scales + p * 2 * groups + column / a.group;
+    for (int base = 0; base < a.width; base += 256) {
+      const int column = base + lane * 8, count = a.width - column;
       float g[8], u[8], da[8], dg[8], du[8], out[8];
-      LoadCodes<Vector>(codes, scales, present ? count : 0, g);
-      LoadCodes<Vector>(codes + a.width, scales + groups, present ? count : 0, u);
-      Load8<T, Vector>(static_cast<const T*>(a.a_grad) + p * a.a_grad_stride + column, present ? count : 0, da);
+      next_g.Values(g);
+      next_u.Values(u);
+      next_da.Values(da);
+      if (base + 256 < a.width) fetch(base + 256);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float s = Sigmoid(g[i]), silu = g[i] * s;
-        const float wda = weight * da[i];
-        dg[i] = wda * u[i] * (s + silu * (1.0f - s));
+        const float wda = weight * da[i], silu_u = silu * u[i];
+        dg[i] = wda * u[i] * fmaf(silu, 1.0f - s, s);
         du[i] = wda * silu;
-        out[i] = weight * silu * u[i];
-        dot += da[i] * silu * u[i];
+        out[i] = weight * silu_u;
+        dot = fmaf(da[i], silu_u, dot);
       }
-      T* h_grad = static_cast<T*>(a.h_grad) + p * 2 * a.width + column;
-      Store8<T, Vector>(h_grad, count, dg);
-      Store8<T, Vector>(h_grad + a.width, count, du);
-      Store8<T, Vector>(static_cast<T*>(a.a) + p * a.width + column, count, out);
+      Store8<T, Vector>(h_row + column, count, dg);
+      Store8<T, Vector>(h_row + a.width + column, count, du);
+      Store8<T, Vector>(out_row + column, count, out);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
@@ -155,55 +219,65 @@ __global__ void __launch_bounds__(kGatedThreads) GatedBackward(GatedArgs a) {
 }
 
 template <typename T, bool Vector>
-__global__ void __launch_bounds__(kGatedThreads) CheckpointLoad(GatedArgs a, T* values, int64_t chunks) {
-  const int lane = threadIdx.x & 31;
-  const int groups = (a.width + a.group - 1) / a.group;
-  const int64_t units = a.rows_count * 2 * chunks, step = int64_t{gridDim.x} * (kGatedThreads / 32);
-  for (int64_t unit = int64_t{blockIdx.x} * (kGatedThreads / 32) + (threadIdx.x >> 5); unit < units; unit += step) {
-    const int64_t half = unit / chunks;   // 2 p for g, 2 p + 1 for u
-    const int column = static_cast<int>(unit - half * chunks) * 256 + lane * 8;
-    float v[8];
-    LoadCodes<Vector>(a.codes + half * a.width + column, a.scales + half * groups + column / a.group,
-                      a.width - column, v);
-    if constexpr (sizeof(T) == 2) {
-      Store8<T, Vector>(values + half * a.width + column, a.width - column, v);
-    } else {
-      Store8<T, false>(values + half * a.width + column, a.width - column, v);
+__global__ void __launch_bounds__(kGatedThreads) CheckpointLoad(GatedArgs a, T* values) {
+  const int lane = threadIdx.x & 31, shift = 31 - __clz(a.group);
+  const int groups = (a.width + a.group - 1) >> shift, stride = static_cast<int>(gridDim.y) * 256;
+  const int64_t halves = a.rows_count * 2, step = int64_t{gridDim.x} * (kGatedThreads / 32);
+  // Half 2 p is row p's gate, 2 p + 1 its up.
+  for (int64_t half = int64_t{blockIdx.x} * (kGatedThreads / 32) + (threadIdx.x >> 5); half < halves; half += step) {
+    const int8_t* code_row = a.codes + half * a.width;
+    const float* scale_row = a.scales + half * groups;
+    const int begin = static_cast<int>(blockIdx.y) * 256;
+    RawCodes<Vector> next;
+    const auto fetch = [&](int base) {
+      const int column = base + lane * 8;
+      next.Fetch(code_row + column, scale_row + (column >> shift), a.width - column);
+    };
+    fetch(begin);
+    for (int base = begin; base < a.width; base += stride) {
+      const int column = base + lane * 8;
+      float v[8];
+      next.Values(v);
+      if (base + stride < a.width) fetch(base + stride);
+      Store8<T, Vector && sizeof(T) == 2>(values + half * a.width + column, a.width - column, v);
     }
   }
 }
 
 bool Aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-unsigned Blocks(int64_t units) {
-  return static_cast<unsigned>(std::min<int64_t>((units + kGatedThreads / 32 - 1) / (kGatedThreads / 32), 1 << 20));
+// A warp per row, and where that leaves the device empty also a part of each
+// row's columns per warp.
+dim3 RowBlocks(int64_t rows, int width) {
+  const int64_t blocks = std::min<int64_t>((rows + kGatedThreads / 32 - 1) / (kGatedThreads / 32), 1 << 20);
+  const int64_t room = int64_t{RoutedSmCount()} * 8 / blocks;   // blocks that run at once, for each of these
+  const int64_t parts = std::min<int64_t>((width + 255) / 256, std::max<int64_t>(1, room));
+  return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(parts, 65535)));
 }
 
 template <typename T>
 void Save(const GatedArgs& a, cudaStream_t stream) {
-  const int64_t chunks = (a.width + 255) / 256;
   const bool vector = a.width % 8 == 0 && a.h_stride % 8 == 0 && Aligned(a.h, 16) && Aligned(a.a, 16) && Aligned(a.codes, 8);
-  const unsigned blocks = Blocks(a.rows_count * chunks);
-  if (vector) GatedSave<T, true><<<blocks, kGatedThreads, 0, stream>>>(a, chunks);
-  else GatedSave<T, false><<<blocks, kGatedThreads, 0, stream>>>(a, chunks);
+  const dim3 blocks = RowBlocks(a.rows_count, a.width);
+  if (vector) GatedSave<T, true><<<blocks, kGatedThreads, 0, stream>>>(a);
+  else GatedSave<T, false><<<blocks, kGatedThreads, 0, stream>>>(a);
 }
 
 template <typename T>
 void Backward(const GatedArgs& a, cudaStream_t stream) {
   const bool vector = a.width % 8 == 0 && a.a_grad_stride % 8 == 0 && Aligned(a.a_grad, 16) && Aligned(a.a, 16) &&
                       Aligned(a.h_grad, 16) && Aligned(a.codes, 8);
-  const unsigned blocks = Blocks(a.rows_count);
+  const unsigned blocks = RowBlocks(a.rows_count, 1).x;
   if (vector) GatedBackward<T, true><<<blocks, kGatedThreads, 0, stream>>>(a);
   else GatedBackward<T, false><<<blocks, kGatedThreads, 0, stream>>>(a);
 }
 
 template <typename T>
 void Load(const GatedArgs& a, void* values, cudaStream_t stream) {
-  const int64_t chunks = (a.width + 255) / 256;
   const bool vector = a.width % 8 == 0 && Aligned(values, 16) && Aligned(a.codes, 8);
-  const unsigned blocks = Blocks(a.rows_count * 2 * chunks);
-  if (vector) CheckpointLoad<T, true><<<blocks, kGatedThreads, 0, stream>>>(a, static_cast<T*>(values), chunks);
-  else CheckpointLoad<T, false><<<blocks, kGatedThreads, 0, stream>>>(a, static_cast<T*>(values), chunks);
+  const dim3 blocks = RowBlocks(a.rows_count * 2, a.width);
+  if (vector) CheckpointLoad<T, true><<<blocks, kGatedThreads, 0, stream>>>(a, static_cast<T*>(values));
+  else CheckpointLoad<T, false><<<blocks, kGatedThreads, 0, stream>>>(a, static_cast<T*>(values));
 }
 
 void Launched() {
