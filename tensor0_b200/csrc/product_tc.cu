@@ -19,8 +19,6 @@
 // bring and not stored.  In the weight gradient they would enter the sum: the
 // matrix warp zeroes them in shared memory, in both operands, so that a value
 // that is not finite stays with its own expert.
-#include <cuda.h>
-
 #include <algorithm>
 
 #include "engine.h"
@@ -28,6 +26,7 @@
 #include "routed.cuh"
 #include "routed.h"
 #include "tcgen05.cuh"
+#include "tensor_map.h"
 
 namespace t0b {
 namespace {
@@ -208,11 +207,9 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
         }
       }
     }
-    if (!ok) {   // given up: the copies in flight land before the block ends
-      const uint32_t pending = fill < Shape::kStages ? fill : Shape::kStages;
-      for (uint32_t f = fill - pending; f < fill; ++f) {
-        BarrierWait(SharedAddress(&s.full[f % Shape::kStages]), (f / Shape::kStages) & 1, nullptr);
-      }
+    // Whoever gives up, the copies in flight land before the block ends.
+    for (uint32_t f = fill - min(fill, static_cast<uint32_t>(Shape::kStages)); f < fill; ++f) {
+      BarrierWait(SharedAddress(&s.full[f % Shape::kStages]), (f / Shape::kStages) & 1, nullptr);
     }
   } else if (warp == 1) {
     // Matrix instructions, issued by lane 0.
@@ -414,50 +411,18 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
   }
 }
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled Encoder() {
-  static const EncodeTiled function = [] {
-    void* entry = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    Check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &found), "tensor map entry point");
-    if (found != cudaDriverEntryPointSuccess || entry == nullptr) {
-      throw std::runtime_error("the driver has no cuTensorMapEncodeTiled");
-    }
-    return reinterpret_cast<EncodeTiled>(entry);
-  }();
-  return function;
-}
-
-// Map of a 16-bit operand [depth, rows, columns] (depth 0: two dimensions)
-// with boxes of 64 columns and `box` rows, 128-byte swizzled.
-void Encode(CUtensorMap* map, bool bf16, const void* data, int64_t columns, int64_t rows, int64_t depth,
-            int64_t row_stride, int64_t depth_stride, int box) {
-  const cuuint64_t sizes[3] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows),
-                               static_cast<cuuint64_t>(depth)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_stride) * 2, static_cast<cuuint64_t>(depth_stride) * 2};
-  const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box), 1}, steps[3] = {1, 1, 1};
-  const CUresult status = Encoder()(
-      map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth != 0 ? 3 : 2,
-      const_cast<void*>(data), sizes, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (status != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed");
-}
-
 template <int kKind, int kWide, bool kGather>
 void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStream_t stream) {
   using Shape = TcShape<kWide>;
   TcArgs a{};
   const int x_width = kKind == kProductTransposed ? p.outer : p.inner;
   if (p.gather_x == 0) {
-    Encode(&a.a, bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kTileRows);
+    a.a = EncodeHalves(bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kTileRows);
   }
   if constexpr (kKind == kProductWeightGrad) {
-    if (p.gather_w == 0) Encode(&a.b, bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
+    if (p.gather_w == 0) a.b = EncodeHalves(bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
   } else {
-    Encode(&a.b, bf16, p.w, p.outer, p.inner, p.experts, p.outer, int64_t{p.inner} * p.outer,
+    a.b = EncodeHalves(bf16, p.w, p.outer, p.inner, p.experts, p.outer, int64_t{p.inner} * p.outer,
            kKind == kProduct ? kDeep : kWide);
   }
   a.a_data = static_cast<const uint16_t*>(p.x);
