@@ -16,7 +16,7 @@
 // Two blocks per streaming multiprocessor walk tasks: some weight rows of one
 // expert and eight of its token rows.  Eight warps compute: 16-row tiles times
 // kParts parts of the deep axis, summed in shared memory in a fixed order.  One
-// warp brings the weights by TMA, three 16 KB stages ahead, and two warps lay
+// warp brings the weights by TMA, three 16 KB stages ahead, and four warps lay
 // out x and the scales of the next 1024 deep values meanwhile, so that the
 // computing warps wait for neither.  (Weights loaded straight into registers
 // touch eight rows per instruction: the load path was the bound at twice the
@@ -39,7 +39,7 @@ constexpr int kMvBox = 256;             // deep values of a row in one box: 128 
 constexpr int kMvStages = 3;
 constexpr uint32_t kMvStageBytes = 16 * kMvWarps * 128;   // kParts boxes of all the block's rows
 constexpr int kMvChunk = 1024;          // deep values of x and of the scales laid out at a time
-constexpr int kMvLayout = 64;           // threads that lay them out
+constexpr int kMvLayout = 128;          // threads that lay them out
 
 // Row stride of x in shared memory, in units of 8 values: 4 more than a
 // multiple of 8, so that two rows' 16-byte reads use different banks.
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
           const int units = (min(kMvChunk, a.inner - k0) + 127) / 128 * 16;
           const int chunk_groups = min(kChunkGroups, groups - k0 / kGroup);
           // Loads first, as many at once as there are registers for.
-          constexpr int kQuads = kChunkGroups / 4, kStep = kMvLayout / kQuads, kLoads = kRows / kStep;
+          constexpr int kQuads = kChunkGroups / 4, kStep = kMvLayout / kQuads, kLoads = (kRows + kStep - 1) / kStep;
           const int quad = lt % kQuads;
           uint2 quads[kLoads < 8 ? kLoads : 8];
           const auto fetch_quads = [&](int from) {
@@ -265,7 +265,9 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
           const auto store_quads = [&](int from) {
 #pragma unroll
             for (int i = 0; i < (kLoads < 8 ? kLoads : 8); ++i) {
-              uint32_t* to = reinterpret_cast<uint32_t*>(scale_out + (lt / kQuads + (from + i) * kStep) * kScaleStride + quad * 4);
+              const int row = lt / kQuads + (from + i) * kStep;
+              if (row >= kRows) break;
+              uint32_t* to = reinterpret_cast<uint32_t*>(scale_out + row * kScaleStride + quad * 4);
               to[0] = quads[i].x;
               to[1] = quads[i].y;
             }
