@@ -22,7 +22,7 @@ latency-bound step allocates nothing.
 
 from __future__ import annotations
 
-import ctypes
+import threading
 from typing import NamedTuple
 
 import torch
@@ -32,6 +32,7 @@ from . import _native
 _HALF = {torch.float16: _native.F16, torch.bfloat16: _native.BF16}
 _FLOAT = {torch.float32: _native.F32, **_HALF}
 _SCORE = {"softmax": 0, "sigmoid": 1}
+_INT, _REAL = torch.int32, torch.float32
 
 
 class Routing(NamedTuple):
@@ -62,30 +63,40 @@ class Int4Weights(NamedTuple):
 
 def _device(*tensors: torch.Tensor) -> int:
     """Index of the CUDA device that holds all the tensors."""
-    index = tensors[0].get_device()
+    index = tensors[0].get_device()   # -1 for host storage
     for tensor in tensors:
-        other = tensor.get_device()   # -1 for host storage
-        if other < 0 or not tensor.is_cuda:
-            raise ValueError("routed storage must be a CUDA tensor (there is no CPU fallback)")
-        if other != index:
+        if tensor.get_device() != index or not tensor.is_cuda:
+            if not tensor.is_cuda or not tensors[0].is_cuda:
+                raise ValueError("routed storage must be a CUDA tensor (there is no CPU fallback)")
             raise ValueError("routed operands must be on one device")
     return index
 
 
 def _packed(tensor: torch.Tensor, shape: tuple, dtype: torch.dtype, what: str) -> int:
-    if tensor.dtype is not dtype or tensor.shape != shape or not tensor.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {list(shape)}, got {tensor.dtype} "
-                         f"{list(tensor.shape)} with strides {list(tensor.stride())}")
-    return tensor.data_ptr()
+    if tensor.dtype is dtype and tensor.shape == shape and tensor.is_contiguous():
+        return tensor.data_ptr()
+    raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {list(shape)}, got {tensor.dtype} "
+                     f"{list(tensor.shape)} with strides {list(tensor.stride())}")
 
 
-def _matrix(tensor: torch.Tensor, what: str) -> int:
-    """Row stride of a 2-d tensor whose rows are contiguous."""
-    rows, width = tensor.shape
-    stride, step = tensor.stride()
+def _output(like: torch.Tensor, out: torch.Tensor | None, shape: tuple) -> tuple[torch.Tensor, int]:
+    """The result of an operator and its address: new, or ``out`` if that fits."""
+    if out is None:
+        out = like.new_empty(shape)
+        return out, out.data_ptr()
+    _device(like, out)
+    return out, _packed(out, shape, like.dtype, "out")
+
+
+def _rows(x: torch.Tensor, rows: int, width: int, what: str, gather: bool = False) -> tuple[int, int]:
+    """(address, row stride) of a matrix of that shape whose rows are contiguous."""
+    if x.shape != (rows, width):
+        kind = "token" if gather else "expert-ordered"
+        raise ValueError(f"{what} must be [{rows}, {width}] ({kind} rows), got {list(x.shape)}")
+    stride, step = x.stride()
     if step != 1 and width > 1:
-        raise ValueError(f"{what} must be 2-d with contiguous rows")
-    return stride if rows > 1 or stride > width else width
+        raise ValueError(f"{what} must have contiguous rows")
+    return x.data_ptr(), stride if rows > 1 or stride > width else width
 
 
 def _code(table: dict, tensor: torch.Tensor, what: str) -> int:
@@ -95,31 +106,54 @@ def _code(table: dict, tensor: torch.Tensor, what: str) -> int:
     return code
 
 
-def _call(name: str, device: int, *arguments) -> None:
-    function = getattr(_native.lib(), name)
-    err = _native.error_buffer()
-    # The stream's handle alone: building a Stream object costs more than the checks.
-    stream = torch._C._cuda_getCurrentRawStream(device)
-    if torch._C._cuda_getDevice() == device:
-        status = function(*arguments, stream, err, len(err))
-    else:
-        with torch.cuda.device(device):
-            status = function(*arguments, stream, err, len(err))
-    if status != 0:
-        _native.check(status, err)
+class _Entry:
+    """A C entry point: called with its arguments up to the stream, on the device's current stream.
+
+    Small operators take less time than their checks, so a call costs as little as it can: the function is looked up
+    once, a thread keeps its error buffer, and the stream is asked for its handle alone.
+    """
+
+    local = threading.local()
+
+    def __init__(self, name: str):
+        self.name = name
+        self.function = None
+
+    def __call__(self, device: int, *arguments) -> None:
+        function = self.function
+        if function is None:
+            function = self.function = getattr(_native.lib(), self.name)
+        try:
+            err = self.local.err
+        except AttributeError:
+            err = self.local.err = _native.error_buffer()
+        stream = torch._C._cuda_getCurrentRawStream(device)
+        if torch._C._cuda_getDevice() == device:
+            status = function(*arguments, stream, err, 512)
+        else:
+            with torch.cuda.device(device):
+                status = function(*arguments, stream, err, 512)
+        if status != 0:
+            _native.check(status, err)
 
 
-def _entries(routing: Routing) -> tuple[int, int, int]:
-    """(tokens, top_k, experts) of a routing whose arrays agree."""
-    if routing.experts.ndim != 2:
+_route, _route_backward = _Entry("t0b_route"), _Entry("t0b_route_backward")
+_product, _weight_grad, _sum = _Entry("t0b_routed_product"), _Entry("t0b_routed_weight_grad"), _Entry("t0b_routed_sum")
+_gated_save, _gated_backward = _Entry("t0b_gated_save"), _Entry("t0b_gated_backward")
+_checkpoint_load, _matvec4 = _Entry("t0b_checkpoint_load"), _Entry("t0b_routed_matvec4")
+
+
+def _entries(routing: Routing) -> tuple[int, int, int, int, int]:
+    """(tokens, top_k, experts, rows, offsets) of a routing whose arrays agree; the last two are addresses."""
+    chosen, _, rows, _, offsets = routing
+    if chosen.dim() != 2:
         raise ValueError("routing experts must be [tokens, top_k]")
-    tokens, top_k = routing.experts.shape
-    _packed(routing.rows, (tokens * top_k,), torch.int32, "routing rows")
-    experts = routing.offsets.numel() - 1
+    tokens, top_k = chosen.shape
+    experts = offsets.numel() - 1
     if experts < 1:
         raise ValueError("routing offsets must be [experts + 1]")
-    _packed(routing.offsets, (experts + 1,), torch.int32, "routing offsets")
-    return tokens, top_k, experts
+    return (tokens, top_k, experts, _packed(rows, (tokens * top_k,), _INT, "routing rows"),
+            _packed(offsets, (experts + 1,), _INT, "routing offsets"))
 
 
 def empty_routing(tokens: int, top_k: int, experts: int, device="cuda") -> Routing:
@@ -149,28 +183,28 @@ def route(logits: torch.Tensor, top_k: int, *, groups: int = 1, top_groups: int 
     (``group_best`` 1) or sum of the two best (2) stay.  ``renormalize`` divides the chosen scores by their sum.
     ``mask`` (bool [tokens]): tokens that are False take no expert, whatever their logits hold.
     """
-    if logits.ndim != 2:
+    if logits.dim() != 2:
         raise ValueError("logits must be [tokens, experts]")
     tokens, experts = logits.shape
-    device = _device(logits, *(t for t in (bias, mask) if t is not None))
+    device = _device(logits, *[t for t in (bias, mask) if t is not None])
     code = _code(_FLOAT, logits, "logits")
-    bias_pointer = None if bias is None else _packed(bias, (experts,), torch.float32, "bias")
+    address, stride = _rows(logits, tokens, experts, "logits")
+    bias_pointer = None if bias is None else _packed(bias, (experts,), _REAL, "bias")
     mask_pointer = None if mask is None else _packed(mask, (tokens,), torch.bool, "mask")
     if out is None:
         out = empty_routing(tokens, top_k, experts, logits.device)
     else:
         _device(logits, *out)
+    chosen, weights, rows, positions, offsets = out
     entry = (tokens, top_k)
-    pointers = (_packed(out.experts, entry, torch.int32, "routing experts"),
-                _packed(out.weights, entry, torch.float32, "routing weights"),
-                _packed(out.rows, (tokens * top_k,), torch.int32, "routing rows"),
-                _packed(out.positions, entry, torch.int32, "routing positions"),
-                _packed(out.offsets, (experts + 1,), torch.int32, "routing offsets"))
     size = _native.lib().t0b_route_workspace(tokens, experts)
-    workspace = logits.new_empty(size, dtype=torch.uint8) if size else None
-    _call("t0b_route", device, code, tokens, experts, top_k, groups, groups if top_groups is None else top_groups,
-          group_best, _score(score), int(renormalize), scale, logits.data_ptr(), _matrix(logits, "logits"),
-          bias_pointer, mask_pointer, *pointers, None if workspace is None else workspace.data_ptr(), size)
+    workspace = logits.new_empty(size, dtype=torch.uint8).data_ptr() if size else None
+    _route(device, code, tokens, experts, top_k, groups, groups if top_groups is None else top_groups, group_best,
+           _score(score), int(renormalize), scale, address, stride, bias_pointer, mask_pointer,
+           _packed(chosen, entry, _INT, "routing experts"), _packed(weights, entry, _REAL, "routing weights"),
+           _packed(rows, (tokens * top_k,), _INT, "routing rows"),
+           _packed(positions, entry, _INT, "routing positions"),
+           _packed(offsets, (experts + 1,), _INT, "routing offsets"), workspace, size)
     return out
 
 
@@ -181,27 +215,19 @@ def route_backward(logits: torch.Tensor, routing: Routing, weights_grad: torch.T
     The choice of experts is piecewise constant and the bias enters it only, so neither has a gradient.  Tokens
     without an expert get zeros, whatever their logits hold.
     """
-    if logits.ndim != 2:
+    if logits.dim() != 2:
         raise ValueError("logits must be [tokens, experts]")
     tokens, experts = logits.shape
     device = _device(logits, routing.experts, weights_grad)
     code = _code(_FLOAT, logits, "logits")
+    address, stride = _rows(logits, tokens, experts, "logits")
     top_k = routing.experts.shape[-1]
-    chosen = _packed(routing.experts, (tokens, top_k), torch.int32, "routing experts")
-    grad = _packed(weights_grad, (tokens, top_k), torch.float32, "weights_grad")
-    if out is None:
-        out = logits.new_empty((tokens, experts))
-    result = _packed(out, (tokens, experts), logits.dtype, "out")
-    _call("t0b_route_backward", device, code, tokens, experts, top_k, _score(score), int(renormalize), scale,
-          logits.data_ptr(), _matrix(logits, "logits"), chosen, grad, result)
+    chosen = _packed(routing.experts, (tokens, top_k), _INT, "routing experts")
+    grad = _packed(weights_grad, (tokens, top_k), _REAL, "weights_grad")
+    out, result = _output(logits, out, (tokens, experts))
+    _route_backward(device, code, tokens, experts, top_k, _score(score), int(renormalize), scale, address, stride,
+                    chosen, grad, result)
     return out
-
-
-def _operand(x: torch.Tensor, width: int, gather: bool, tokens: int, top_k: int, what: str) -> None:
-    rows = tokens if gather else tokens * top_k
-    if x.ndim != 2 or x.shape[0] != rows or x.shape[1] != width:
-        raise ValueError(f"{what} must be [{rows}, {width}] ({'token' if gather else 'expert-ordered'} rows), "
-                         f"got {list(x.shape)}")
 
 
 def routed_matmul(x: torch.Tensor, w: torch.Tensor, routing: Routing, *, gather: bool = False,
@@ -211,23 +237,19 @@ def routed_matmul(x: torch.Tensor, w: torch.Tensor, routing: Routing, *, gather:
     ``w`` [experts, inner, outer], float16 or bfloat16 as ``x``.  ``x`` holds token rows with ``gather`` (row p reads
     its entry's token), else expert-ordered rows.  Summed in 32 bits, rounded once; rows without an expert are zero.
     """
-    tokens, top_k, experts = _entries(routing)
+    tokens, top_k, experts, rows, offsets = _entries(routing)
     device = _device(x, w, routing.rows, routing.offsets)
     code = _code(_HALF, x, "product operands")
-    if w.ndim != 3 or w.shape[0] != experts:
+    if w.dim() != 3 or w.shape[0] != experts:
         raise ValueError(f"weights must be [{experts}, inner, outer]")
     _, inner, outer = w.shape
+    entries = tokens * top_k
+    x_rows = tokens if gather else entries
     weights = _packed(w, w.shape, x.dtype, "weights")
-    _operand(x, outer if transpose else inner, gather, tokens, top_k, "x")
-    width = inner if transpose else outer
-    if out is None:
-        out = x.new_empty((tokens * top_k, width))
-    else:
-        _device(x, out)
-    result = _packed(out, (tokens * top_k, width), x.dtype, "out")
-    _call("t0b_routed_product", device, code, int(transpose), tokens * top_k, experts, top_k, inner, outer,
-          int(gather), x.data_ptr(), x.shape[0], _matrix(x, "x"), weights, routing.rows.data_ptr(),
-          routing.offsets.data_ptr(), result)
+    address, stride = _rows(x, x_rows, outer if transpose else inner, "x", gather)
+    out, result = _output(x, out, (entries, inner if transpose else outer))
+    _product(device, code, int(transpose), entries, experts, top_k, inner, outer, int(gather), address, x_rows, stride,
+             weights, rows, offsets, result)
     return out
 
 
@@ -238,42 +260,34 @@ def routed_weight_grad(x: torch.Tensor, y_grad: torch.Tensor, routing: Routing, 
     Either operand holds token rows (``gather_x``, ``gather_y``) or expert-ordered ones.  An expert without rows
     gets zeros.
     """
-    tokens, top_k, experts = _entries(routing)
+    tokens, top_k, experts, rows, offsets = _entries(routing)
     device = _device(x, y_grad, routing.rows, routing.offsets)
     code = _code(_HALF, x, "product operands")
     if y_grad.dtype != x.dtype:
         raise ValueError("product operands must share a dtype")
     inner, outer = x.shape[-1], y_grad.shape[-1]
-    _operand(x, inner, gather_x, tokens, top_k, "x")
-    _operand(y_grad, outer, gather_y, tokens, top_k, "y_grad")
-    if out is None:
-        out = x.new_empty((experts, inner, outer))
-    else:
-        _device(x, out)
-    result = _packed(out, (experts, inner, outer), x.dtype, "out")
-    _call("t0b_routed_weight_grad", device, code, tokens * top_k, experts, top_k, inner, outer, int(gather_x),
-          x.data_ptr(), x.shape[0], _matrix(x, "x"), int(gather_y), y_grad.data_ptr(), y_grad.shape[0],
-          _matrix(y_grad, "y_grad"), routing.rows.data_ptr(), routing.offsets.data_ptr(), result)
+    entries = tokens * top_k
+    x_rows, y_rows = tokens if gather_x else entries, tokens if gather_y else entries
+    x_address, x_stride = _rows(x, x_rows, inner, "x", gather_x)
+    y_address, y_stride = _rows(y_grad, y_rows, outer, "y_grad", gather_y)
+    out, result = _output(x, out, (experts, inner, outer))
+    _weight_grad(device, code, entries, experts, top_k, inner, outer, int(gather_x), x_address, x_rows, x_stride,
+                 int(gather_y), y_address, y_rows, y_stride, rows, offsets, result)
     return out
 
 
 def routed_sum(y: torch.Tensor, routing: Routing, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """Each token's sum over its experts' rows: [tokens, width].  Also the gradient of gathering token rows."""
-    if routing.positions.ndim != 2:
+    if routing.positions.dim() != 2:
         raise ValueError("routing positions must be [tokens, top_k]")
     tokens, top_k = routing.positions.shape
     device = _device(y, routing.positions)
     code = _code(_HALF, y, "sum operands")
-    positions = _packed(routing.positions, (tokens, top_k), torch.int32, "routing positions")
-    if y.ndim != 2 or y.shape[0] != tokens * top_k:
-        raise ValueError(f"y must be [{tokens * top_k}, width]")
-    width = y.shape[1]
-    if out is None:
-        out = y.new_empty((tokens, width))
-    else:
-        _device(y, out)
-    result = _packed(out, (tokens, width), y.dtype, "out")
-    _call("t0b_routed_sum", device, code, tokens, top_k, width, y.data_ptr(), _matrix(y, "y"), positions, result)
+    positions = _packed(routing.positions, (tokens, top_k), _INT, "routing positions")
+    width = y.shape[-1]
+    address, stride = _rows(y, tokens * top_k, width, "y")
+    out, result = _output(y, out, (tokens, width))
+    _sum(device, code, tokens, top_k, width, address, stride, positions, result)
     return out
 
 
@@ -281,11 +295,10 @@ def _row_weights(routing: Routing | None, rows: int) -> tuple:
     """(weights, rows, offsets, experts) arguments of the gated entry points."""
     if routing is None:
         return None, None, None, 0
-    tokens, top_k, experts = _entries(routing)
+    tokens, top_k, experts, entries, offsets = _entries(routing)
     if tokens * top_k != rows:
         raise ValueError(f"the routing has {tokens * top_k} entries, the activation {rows} rows")
-    weights = _packed(routing.weights, (tokens, top_k), torch.float32, "routing weights")
-    return weights, routing.rows.data_ptr(), routing.offsets.data_ptr(), experts
+    return _packed(routing.weights, (tokens, top_k), _REAL, "routing weights"), entries, offsets, experts
 
 
 def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 128,
@@ -295,7 +308,7 @@ def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 
     ``group`` (32, 64 or 128) neighbours of one half share a scale, their largest magnitude / 127.  A row's weight is
     its entry's in ``routing``, or 1 without one; with one, rows without an expert are not read and give zeros.
     """
-    if h.ndim != 2 or h.shape[1] % 2 or h.shape[1] == 0:
+    if h.dim() != 2 or h.shape[1] % 2 or h.shape[1] == 0:
         raise ValueError("h must be [rows, 2 * width]")
     rows, width = h.shape[0], h.shape[1] // 2
     device = _device(h, *(() if routing is None else (routing.weights, routing.rows, routing.offsets)))
@@ -303,6 +316,7 @@ def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 
     if group not in (32, 64, 128):
         raise ValueError("checkpoint group must be 32, 64 or 128")
     scales = 2 * -(-width // group)
+    address, stride = _rows(h, rows, 2 * width, "h")
     if out is None:
         a = h.new_empty((rows, width))
         kept = Checkpoint(h.new_empty((rows, 2 * width), dtype=torch.int8),
@@ -312,10 +326,10 @@ def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 
         if kept.group != group:
             raise ValueError("out's checkpoint has another group")
         _device(h, a, kept.codes, kept.scales)
-    _call("t0b_gated_save", device, code, rows, width, group, h.data_ptr(), _matrix(h, "h"),
-          *_row_weights(routing, rows), _packed(a, (rows, width), h.dtype, "out"),
-          _packed(kept.codes, (rows, 2 * width), torch.int8, "checkpoint codes"),
-          _packed(kept.scales, (rows, scales), torch.float32, "checkpoint scales"))
+    _gated_save(device, code, rows, width, group, address, stride, *_row_weights(routing, rows),
+                _packed(a, (rows, width), h.dtype, "out"),
+                _packed(kept.codes, (rows, 2 * width), torch.int8, "checkpoint codes"),
+                _packed(kept.scales, (rows, scales), _REAL, "checkpoint scales"))
     return a, kept
 
 
@@ -324,11 +338,11 @@ def _checkpoint(checkpoint: Checkpoint) -> tuple[int, int, int, int]:
     codes, scales, group = checkpoint
     if group not in (32, 64, 128):
         raise ValueError("checkpoint group must be 32, 64 or 128")
-    if codes.ndim != 2 or codes.shape[1] % 2 or codes.shape[1] == 0:
+    if codes.dim() != 2 or codes.shape[1] % 2 or codes.shape[1] == 0:
         raise ValueError("checkpoint codes must be [rows, 2 * width]")
     rows, width = codes.shape[0], codes.shape[1] // 2
     return (rows, width, _packed(codes, codes.shape, torch.int8, "checkpoint codes"),
-            _packed(scales, (rows, 2 * -(-width // group)), torch.float32, "checkpoint scales"))
+            _packed(scales, (rows, 2 * -(-width // group)), _REAL, "checkpoint scales"))
 
 
 def gated_backward(checkpoint: Checkpoint, a_grad: torch.Tensor, *, routing: Routing | None = None,
@@ -343,14 +357,13 @@ def gated_backward(checkpoint: Checkpoint, a_grad: torch.Tensor, *, routing: Rou
     device = _device(a_grad, checkpoint.codes, checkpoint.scales,
                      *(() if routing is None else (routing.weights, routing.rows, routing.offsets)))
     code = _code(_HALF, a_grad, "gated activations")
-    if a_grad.shape != (rows, width):
-        raise ValueError(f"a_grad must be [{rows}, {width}]")
+    address, stride = _rows(a_grad, rows, width, "a_grad")
     weights = _row_weights(routing, rows)
     h_grad = a_grad.new_empty((rows, 2 * width))
     a = a_grad.new_empty((rows, width))
     weights_grad = a_grad.new_empty((rows,) if routing is None else routing.weights.shape, dtype=torch.float32)
-    _call("t0b_gated_backward", device, code, rows, width, checkpoint.group, codes, scales, a_grad.data_ptr(),
-          _matrix(a_grad, "a_grad"), *weights, h_grad.data_ptr(), a.data_ptr(), weights_grad.data_ptr())
+    _gated_backward(device, code, rows, width, checkpoint.group, codes, scales, address, stride, *weights,
+                    h_grad.data_ptr(), a.data_ptr(), weights_grad.data_ptr())
     return h_grad, a, weights_grad
 
 
@@ -361,15 +374,15 @@ def checkpoint_load(checkpoint: Checkpoint, dtype: torch.dtype = torch.float32) 
     if dtype not in _FLOAT:
         raise ValueError("checkpoints load as float32, float16 or bfloat16")
     values = checkpoint.codes.new_empty((rows, 2 * width), dtype=dtype)
-    _call("t0b_checkpoint_load", device, _FLOAT[dtype], rows, width, checkpoint.group, codes, scales,
-          values.data_ptr())
+    _checkpoint_load(device, _FLOAT[dtype], rows, width, checkpoint.group, codes, scales,
+                     values.data_ptr())
     return values
 
 
 def pack_int4(w: torch.Tensor, group: int = 128) -> Int4Weights:
     """``w`` [experts, inner, outer] in 4 bits: per group of ``group`` inner neighbours the scale max|w| / 7 (in w's
     type) and whole numbers from -7 to 7.  Done once per model, in plain torch."""
-    if w.ndim != 3 or w.dtype not in _HALF:
+    if w.dim() != 3 or w.dtype not in _HALF:
         raise ValueError("weights must be [experts, inner, outer] of float16 or bfloat16")
     if group not in (32, 64, 128) or w.shape[1] % group:
         raise ValueError("weight group must be 32, 64 or 128 and divide the inner width")
@@ -387,25 +400,22 @@ def routed_matvec(x: torch.Tensor, weights: Int4Weights, routing: Routing, *, ga
 
     Memory bound on the weights: each chosen expert's are read once however many rows it has.
     """
-    tokens, top_k, experts = _entries(routing)
+    tokens, top_k, experts, rows, offsets = _entries(routing)
     codes, scales, group = weights
     device = _device(x, codes, scales, routing.rows, routing.offsets)
     code = _code(_HALF, x, "4-bit product operands")
-    if group not in (32, 64, 128) or x.ndim != 2 or x.shape[1] % group:
+    if group not in (32, 64, 128) or x.dim() != 2 or x.shape[1] % group:
         raise ValueError("weight group must be 32, 64 or 128 and divide the inner width")
     inner = x.shape[1]
-    if codes.ndim != 3:
+    if codes.dim() != 3:
         raise ValueError("4-bit weight codes must be [experts, outer, inner / 2]")
     outer = codes.shape[1]
     code_pointer = _packed(codes, (experts, outer, inner // 2), torch.uint8, "4-bit weight codes")
     scale_pointer = _packed(scales, (experts, outer, inner // group), x.dtype, "4-bit weight scales")
-    _operand(x, inner, gather, tokens, top_k, "x")
-    if out is None:
-        out = x.new_empty((tokens * top_k, outer))
-    else:
-        _device(x, out)
-    result = _packed(out, (tokens * top_k, outer), x.dtype, "out")
-    _call("t0b_routed_matvec4", device, code, tokens * top_k, experts, top_k, inner, outer, group, int(gather),
-          x.data_ptr(), x.shape[0], _matrix(x, "x"), code_pointer, scale_pointer, routing.rows.data_ptr(),
-          routing.offsets.data_ptr(), result)
+    entries = tokens * top_k
+    x_rows = tokens if gather else entries
+    address, stride = _rows(x, x_rows, inner, "x", gather)
+    out, result = _output(x, out, (entries, outer))
+    _matvec4(device, code, entries, experts, top_k, inner, outer, group, int(gather), address, x_rows, stride,
+             code_pointer, scale_pointer, rows, offsets, result)
     return out
