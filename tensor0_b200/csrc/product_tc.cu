@@ -237,10 +237,11 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
         if constexpr (kKind == kProductWeightGrad) {
           const int valid = t.count - k * kDeep;
           if (valid < kDeep) {   // rows of the next expert: zero, in every column block of both operands
-            const int blocks = 2 + kWide / 64, chunks = (kDeep - valid) * 8;
-            for (int i = lane; i < blocks * chunks; i += 32) {
-              const uint32_t at = a_smem + (i / chunks) * kBlockBytes + valid * kSwizzleRow + (i % chunks) * 16;
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+            for (int block = 0; block < 2 + kWide / 64; ++block) {
+              const uint32_t to = a_smem + (block + 1) * kBlockBytes;
+              for (uint32_t at = to - (kDeep - valid) * kSwizzleRow + lane * 16; at < to; at += 512) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+              }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -352,10 +353,10 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
       const TcTile t = walk.At(tile);
       const int slices = walk.Slices(t), last = t.begin + t.count - 1;
       const uint16_t* source[8];   // the tile's rows (products)
-      int64_t next[4];             // the next slice's token rows (weight gradient)
+      int next[4];                 // entries of the next slice's rows (weight gradient), used a slice later
       auto slice_rows = [&](int k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) next[i] = a.rows[min(t.begin + k * kDeep + r0 + 16 * i, last)] / a.top_k;
+        for (int i = 0; i < 4; ++i) next[i] = a.rows[min(t.begin + k * kDeep + r0 + 16 * i, last)];
       };
       if constexpr (kKind != kProductWeightGrad) {
 #pragma unroll
@@ -381,7 +382,8 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
         } else {
           int64_t row[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) row[i] = next[i];
+          for (int i = 0; i < 4; ++i) row[i] = next[i] / a.top_k;
+          if (k + 1 < slices) slice_rows(k + 1);
           auto copy = [&](uint32_t tile_smem, const uint16_t* data, int64_t rows, int64_t stride, int column, int columns,
                           int blocks) {
             for (int block = 0; block < blocks; ++block) {
@@ -396,7 +398,6 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
           };
           if (a.gather_a != 0) copy(a_smem, a.a_data, a.a_rows, a.a_stride, t.m0, a.inner, 2);
           if (a.gather_b != 0) copy(b_smem, a.b_data, a.b_rows, a.b_stride, t.n0, a.outer, kWide / 64);
-          if (k + 1 < slices) slice_rows(k + 1);
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];"
                      ::"r"(SharedAddress(&s.full[stage])) : "memory");
