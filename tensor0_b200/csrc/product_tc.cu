@@ -15,8 +15,8 @@
 //   transposed:  A = rows of x (deep-major), B = W[e]^T: W[e] as it lies (deep-major)
 //   weight grad: A = x^T, B = y: rows are the deep axis, both as they lie (wide-major)
 //
-// A tile's rows past its expert's last are computed from whatever the loads
-// bring and not stored.  In the weight gradient they would enter the sum: the
+// A tile's rows past its expert's last are computed from whatever lies in
+// shared memory and not stored (experts with few rows load few).  In the weight gradient they would enter the sum: the
 // matrix warp zeroes them in shared memory, in both operands, so that a value
 // that is not finite stays with its own expert.
 #include <algorithm>
@@ -31,7 +31,7 @@
 namespace t0b {
 namespace {
 
-constexpr int kTileRows = 128, kDeep = 64;
+constexpr int kTileRows = 128, kDeep = 64, kRowBox = 32;   // kRowBox: rows of x that one copy brings
 constexpr int kTcThreads = 192, kGatherThreads = 128;      // roles; copying threads where rows are gathered
 constexpr uint32_t kSwizzleRow = 128;                      // bytes of 64 16-bit values
 constexpr uint32_t kABytes = kTileRows * kSwizzleRow;      // one stage of A
@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
       // Column blocks of 64 that lie in the operand at all.
       const int a_blocks = kKind == kProductWeightGrad ? min(2, (a.inner - t.m0 + 63) / 64) : 1;
       const int b_blocks = min(kWide / 64, (width - t.n0 + 63) / 64);
-      const uint32_t a_bytes = kKind == kProductWeightGrad ? a_blocks * kBlockBytes : kABytes;
+      const int row_boxes = (min(kTileRows, t.count - t.m0) + kRowBox - 1) / kRowBox;   // products
+      const uint32_t a_bytes = kKind == kProductWeightGrad ? a_blocks * kBlockBytes : row_boxes * (kRowBox * kSwizzleRow);
       const uint32_t b_bytes = kKind == kProductTransposed ? Shape::kBBytes : b_blocks * kBlockBytes;
       const bool load_a = !kGather || a.gather_a == 0, load_b = !kGather || a.gather_b == 0;
       const uint32_t bytes = (load_a ? a_bytes : 0) + (load_b ? b_bytes : 0);
@@ -198,7 +199,9 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
             LoadTile2(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, t.begin + k0);
           }
         } else {
-          if (load_a && lane == 0) LoadTile2(a_smem, &a.a, full, k0, t.begin + t.m0);
+          if (load_a && lane < row_boxes) {
+            LoadTile2(a_smem + lane * (kRowBox * kSwizzleRow), &a.a, full, k0, t.begin + t.m0 + lane * kRowBox);
+          }
           if constexpr (kKind == kProduct) {
             if (lane < b_blocks) LoadTile3(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, k0, t.e);
           } else {
@@ -352,7 +355,8 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
     for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
       const TcTile t = walk.At(tile);
       const int slices = walk.Slices(t), last = t.begin + t.count - 1;
-      const uint16_t* source[8];   // the tile's rows (products)
+      const int valid = t.count - t.m0;   // rows of the tile (products)
+      const uint16_t* source[8];          // where they lie
       int next[4];                 // entries of the next slice's rows (weight gradient), used a slice later
       auto slice_rows = [&](int k) {
 #pragma unroll
@@ -378,7 +382,9 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
           const int deep = kKind == kProduct ? a.inner : a.outer;
           const bool inside = k * kDeep + c * 8 < deep;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) CopyChunk(a_smem, r0 + 16 * i, c, inside ? source[i] + k * kDeep : a.a_data, inside);
+          for (int i = 0; i < 8; ++i) {
+            if (r0 + 16 * i < valid) CopyChunk(a_smem, r0 + 16 * i, c, inside ? source[i] + k * kDeep : a.a_data, inside);
+          }
         } else {
           int64_t row[4];
 #pragma unroll
@@ -418,7 +424,7 @@ void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStrea
   TcArgs a{};
   const int x_width = kKind == kProductTransposed ? p.outer : p.inner;
   if (p.gather_x == 0) {
-    a.a = EncodeHalves(bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kTileRows);
+    a.a = EncodeHalves(bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kRowBox);
   }
   if constexpr (kKind == kProductWeightGrad) {
     if (p.gather_w == 0) a.b = EncodeHalves(bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
@@ -466,8 +472,13 @@ void ByWidth(const ProductArgs& p, bool bf16, cudaStream_t stream) {
     if (p.gather_x != 0 || p.gather_w != 0) LaunchTc<kKind, kWide, true>(p, bf16, tiles(kWide), sms, stream);
     else LaunchTc<kKind, kWide, false>(p, bf16, tiles(kWide), sms, stream);
   };
-  if (tiles(256) >= sms) launch(std::integral_constant<int, 256>{});
-  else if (tiles(128) >= sms) launch(std::integral_constant<int, 128>{});
+  // The widest tile that still gives every other multiprocessor one: what a
+  // block brings per slice grows with the width, and narrow tiles bring the
+  // rows of x more often (512 rows of 64 experts, 1024 x 1024: 27 us with 256
+  // columns, 32 with 128, 48 with 64; one row of 8 experts, 512 x 512: 8.1, 7.1
+  // and 6.7 us).
+  if (2 * tiles(256) >= sms) launch(std::integral_constant<int, 256>{});
+  else if (2 * tiles(128) >= sms) launch(std::integral_constant<int, 128>{});
   else launch(std::integral_constant<int, 64>{});
 }
 
