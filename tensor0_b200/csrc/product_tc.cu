@@ -40,7 +40,11 @@ constexpr int kMaxStages = 8;
 constexpr uint32_t kStagingBytes = 32 * kSwizzleRow;       // of one storing warp
 
 struct TcArgs {
-  CUtensorMap a, b;
+  // a_few: products, kRowBox rows at a time.  Wide-major operands whose width
+  // is whole blocks of 64 columns have one box for all of a tile's blocks
+  // (blocked): a copy costs by its number as well as by its bytes.
+  CUtensorMap a, a_few, b;
+  int a_blocked, b_blocked;
   const uint16_t *a_data, *b_data;   // gathered operands
   int64_t a_rows, a_stride, b_rows, b_stride;
   const int32_t* rows;
@@ -176,8 +180,10 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
       const int a_blocks = kKind == kProductWeightGrad ? min(2, (a.inner - t.m0 + 63) / 64) : 1;
       const int b_blocks = min(kWide / 64, (width - t.n0 + 63) / 64);
       const int row_boxes = (min(kTileRows, t.count - t.m0) + kRowBox - 1) / kRowBox;   // products
-      const uint32_t a_bytes = kKind == kProductWeightGrad ? a_blocks * kBlockBytes : row_boxes * (kRowBox * kSwizzleRow);
-      const uint32_t b_bytes = kKind == kProductTransposed ? Shape::kBBytes : b_blocks * kBlockBytes;
+      const uint32_t a_bytes = kKind != kProductWeightGrad ? row_boxes * (kRowBox * kSwizzleRow)
+                               : a.a_blocked != 0          ? kABytes
+                                                           : a_blocks * kBlockBytes;
+      const uint32_t b_bytes = kKind == kProductTransposed || a.b_blocked != 0 ? Shape::kBBytes : b_blocks * kBlockBytes;
       const bool load_a = !kGather || a.gather_a == 0, load_b = !kGather || a.gather_b == 0;
       const uint32_t bytes = (load_a ? a_bytes : 0) + (load_b ? b_bytes : 0);
       for (int k = 0; k < slices; ++k, ++fill) {
@@ -192,18 +198,34 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
         if (lane == 0) BarrierExpect(full, bytes);
         __syncwarp();
         if constexpr (kKind == kProductWeightGrad) {
-          if (load_a && lane < a_blocks) {
-            LoadTile2(a_smem + lane * kBlockBytes, &a.a, full, t.m0 + lane * 64, t.begin + k0);
+          if (load_a) {
+            if (a.a_blocked != 0) {
+              if (lane == 0) LoadTile3(a_smem, &a.a, full, 0, t.begin + k0, t.m0 / 64);
+            } else if (lane < a_blocks) {
+              LoadTile2(a_smem + lane * kBlockBytes, &a.a, full, t.m0 + lane * 64, t.begin + k0);
+            }
           }
-          if (load_b && lane < b_blocks) {
-            LoadTile2(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, t.begin + k0);
+          if (load_b) {
+            if (a.b_blocked != 0) {
+              if (lane == 0) LoadTile3(b_smem, &a.b, full, 0, t.begin + k0, t.n0 / 64);
+            } else if (lane < b_blocks) {
+              LoadTile2(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, t.begin + k0);
+            }
           }
         } else {
-          if (load_a && lane < row_boxes) {
-            LoadTile2(a_smem + lane * (kRowBox * kSwizzleRow), &a.a, full, k0, t.begin + t.m0 + lane * kRowBox);
+          if (load_a) {
+            if (row_boxes == kTileRows / kRowBox) {
+              if (lane == 0) LoadTile2(a_smem, &a.a, full, k0, t.begin + t.m0);
+            } else if (lane < row_boxes) {
+              LoadTile2(a_smem + lane * (kRowBox * kSwizzleRow), &a.a_few, full, k0, t.begin + t.m0 + lane * kRowBox);
+            }
           }
           if constexpr (kKind == kProduct) {
-            if (lane < b_blocks) LoadTile3(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, k0, t.e);
+            if (a.b_blocked != 0) {
+              if (lane == 0) LoadTile4(b_smem, &a.b, full, 0, k0, t.n0 / 64, t.e);
+            } else if (lane < b_blocks) {
+              LoadTile3(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, k0, t.e);
+            }
           } else {
             if (lane == 0) LoadTile3(b_smem, &a.b, full, k0, t.n0, t.e);
           }
@@ -424,13 +446,25 @@ void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStrea
   TcArgs a{};
   const int x_width = kKind == kProductTransposed ? p.outer : p.inner;
   if (p.gather_x == 0) {
-    a.a = EncodeHalves(bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kKind == kProductWeightGrad ? kDeep : kRowBox);
+    if constexpr (kKind == kProductWeightGrad) {
+      a.a_blocked = p.inner % 64 == 0 ? 1 : 0;
+      a.a = a.a_blocked != 0 ? EncodeBlocks(bf16, p.x, p.inner, p.x_rows, 0, p.x_stride, 0, kDeep, kTileRows / 64)
+                             : EncodeHalves(bf16, p.x, p.inner, p.x_rows, 0, p.x_stride, 0, kDeep);
+    } else {
+      a.a = EncodeHalves(bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kTileRows);
+      a.a_few = EncodeHalves(bf16, p.x, x_width, p.x_rows, 0, p.x_stride, 0, kRowBox);
+    }
   }
+  const int64_t matrix = int64_t{p.inner} * p.outer;
+  a.b_blocked = kKind != kProductTransposed && p.outer % 64 == 0 ? 1 : 0;
   if constexpr (kKind == kProductWeightGrad) {
-    if (p.gather_w == 0) a.b = EncodeHalves(bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
+    if (p.gather_w != 0) a.b_blocked = 0;
+    else if (a.b_blocked != 0) a.b = EncodeBlocks(bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep, kWide / 64);
+    else a.b = EncodeHalves(bf16, p.w, p.outer, p.w_rows, 0, p.w_stride, 0, kDeep);
+  } else if (a.b_blocked != 0) {
+    a.b = EncodeBlocks(bf16, p.w, p.outer, p.inner, p.experts, p.outer, matrix, kDeep, kWide / 64);
   } else {
-    a.b = EncodeHalves(bf16, p.w, p.outer, p.inner, p.experts, p.outer, int64_t{p.inner} * p.outer,
-           kKind == kProduct ? kDeep : kWide);
+    a.b = EncodeHalves(bf16, p.w, p.outer, p.inner, p.experts, p.outer, matrix, kKind == kProduct ? kDeep : kWide);
   }
   a.a_data = static_cast<const uint16_t*>(p.x);
   a.a_rows = p.x_rows;

@@ -65,6 +65,12 @@ __device__ __forceinline__ void LoadTile3(uint32_t dst, const void* map, uint32_
       ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
+__device__ __forceinline__ void LoadTile4(uint32_t dst, const void* map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
 // Shared-memory matrix descriptors of 128-byte swizzled tiles of 16-bit values.
 // Deep-major (K-major): rows of 64 deep values, 8-row atoms 1024 bytes apart.
 // Wide-major (MN-major): 64 neighbours of one deep index per 128 bytes, 8 deep
