@@ -16,7 +16,7 @@ using t0b::Guard;
 using t0b::InvalidArgument;
 
 constexpr int64_t kMaxEntries = (int64_t{1} << 31) - 1;
-constexpr int32_t kMaxWidth = 1 << 24;
+constexpr int32_t kMaxWidth = 1 << 23;   // blocks of 256 columns fit a grid axis
 
 uint64_t Half(int32_t dtype, const char* what) {
   if (dtype != T0B_F16 && dtype != T0B_BF16) throw InvalidArgument(std::string(what) + " take F16 or BF16");
@@ -32,6 +32,7 @@ void Require(bool condition, const char* message) {
 uint64_t Operand(const void* data, int64_t rows, int64_t width, int64_t stride, uint64_t item, const char* what) {
   if (rows < 0 || width < 0) throw InvalidArgument(std::string(what) + " sizes must be nonnegative");
   if (stride < width) throw InvalidArgument(std::string(what) + " row stride is below the row's width");
+  if (stride > kMaxEntries) throw InvalidArgument(std::string(what) + " row stride must be at most 2^31 - 1");
   if (rows == 0 || width == 0) return 0;
   if (data == nullptr) throw InvalidArgument(std::string(what) + " buffer is null");
   if (reinterpret_cast<uintptr_t>(data) % item != 0) {
@@ -86,7 +87,7 @@ uint64_t RequireScore(int32_t dtype, int64_t tokens, int32_t experts, int32_t to
 }
 
 void RequireGroup(int32_t width, int32_t group) {
-  Require(width >= 1 && width <= kMaxWidth, "gated width must be from 1 to 2^24");
+  Require(width >= 1 && width <= kMaxWidth, "gated width must be from 1 to 2^23");
   Require(group == 32 || group == 64 || group == 128, "checkpoint group must be 32, 64 or 128");
 }
 
@@ -107,7 +108,7 @@ uint64_t RequireRowWeights(const float* weights, const int32_t* row_entries, con
 void Product(int kind, int32_t dtype, const t0b::ProductArgs& a, uint64_t out_width, int64_t out_rows, void* stream) {
   RequireRouting(a.entries, a.experts, a.top_k);
   Require(a.inner >= 1 && a.outer >= 1 && a.inner <= kMaxWidth && a.outer <= kMaxWidth,
-          "product widths must be from 1 to 2^24");
+          "product widths must be from 1 to 2^23");
   Require((a.gather_x == 0 || a.gather_x == 1) && (a.gather_w == 0 || a.gather_w == 1), "gather must be zero or one");
   const uint64_t item = Half(dtype, "routed products");
   const int64_t matrices = int64_t{a.experts} * a.inner;
@@ -279,7 +280,7 @@ int t0b_routed_sum(int32_t dtype, int64_t tokens, int32_t top_k, int32_t width, 
     Require(tokens >= 0, "token count must be nonnegative");
     Require(top_k >= 1 && top_k <= t0b::kRouteMaxTopK, "top_k must be from 1 to 32");
     Require(tokens <= kMaxEntries / top_k, "routed entries must be at most 2^31 - 1");
-    Require(width >= 1 && width <= kMaxWidth, "sum width must be from 1 to 2^24");
+    Require(width >= 1 && width <= kMaxWidth, "sum width must be from 1 to 2^23");
     const int64_t entries = tokens * top_k;
     const uint64_t y_bytes = Operand(y, entries, width, y_stride, item, "sum");
     const uint64_t position_bytes = Packed(positions, entries, 1, 4, "position");
@@ -400,7 +401,7 @@ int t0b_routed_matvec4(int32_t dtype, int64_t entries, int32_t experts, int32_t 
     const uint64_t item = Half(dtype, "4-bit products");
     RequireRouting(entries, experts, top_k);
     Require(group == 32 || group == 64 || group == 128, "weight group must be 32, 64 or 128");
-    Require(inner >= 1 && outer >= 1 && inner <= kMaxWidth && outer <= kMaxWidth, "product widths must be from 1 to 2^24");
+    Require(inner >= 1 && outer >= 1 && inner <= kMaxWidth && outer <= kMaxWidth, "product widths must be from 1 to 2^23");
     Require(inner % group == 0, "weight groups must divide the inner width");
     Require(gather == 0 || gather == 1, "gather must be zero or one");
     Require(x_rows == (gather != 0 ? entries / top_k : entries), "an operand has one row per token (gather) or entry");

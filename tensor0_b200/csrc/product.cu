@@ -105,24 +105,28 @@ __global__ void __launch_bounds__(kGenThreads) GeneralProduct(ProductArgs a, int
   }
 }
 
-// A warp sums 256 columns of one token; memory bound, each row read once.
+// A warp sums 256 columns (blockIdx.y) of one token; memory bound, each row
+// read once, four rows in flight.
 template <typename T, bool Vector>
-__global__ void __launch_bounds__(256) RoutedSum(RoutedSumArgs a, int64_t chunks) {
-  const int lane = threadIdx.x & 31;
-  const int64_t units = a.tokens * chunks, step = int64_t{gridDim.x} * 8;
-  for (int64_t u = int64_t{blockIdx.x} * 8 + (threadIdx.x >> 5); u < units; u += step) {
-    const int64_t t = u / chunks;
-    const int column = static_cast<int>(u - t * chunks) * 256 + lane * 8;
-    const int count = a.width - column;
+__global__ void __launch_bounds__(256) RoutedSum(RoutedSumArgs a) {
+  const int column = static_cast<int>(blockIdx.y) * 256 + (threadIdx.x & 31) * 8, count = a.width - column;
+  const T* y = static_cast<const T*>(a.y) + column;
+  const int64_t step = int64_t{gridDim.x} * 8;
+  for (int64_t t = int64_t{blockIdx.x} * 8 + (threadIdx.x >> 5); t < a.tokens; t += step) {
     float sum[8] = {};
-#pragma unroll 4
-    for (int n = 0; n < a.top_k; ++n) {
-      const int p = a.positions[t * a.top_k + n];
-      if (p < 0 || p >= a.entries) continue;
-      float v[8];
-      Load8<T, Vector>(static_cast<const T*>(a.y) + int64_t{p} * a.y_stride + column, count, v);
+    for (int n0 = 0; n0 < a.top_k; n0 += 4) {
+      float v[4][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += v[i];
+      for (int n = 0; n < 4; ++n) {
+        const int64_t p = n0 + n < a.top_k ? a.positions[t * a.top_k + n0 + n] : -1;
+        const bool some = p >= 0 && p < a.entries;
+        Load8<T, Vector>(y + (some ? p : 0) * a.y_stride, some ? count : 0, v[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] += v[n][i];
+      }
     }
     Store8<T, Vector>(static_cast<T*>(a.out) + t * a.out_stride + column, count, sum);
   }
@@ -138,12 +142,12 @@ void Launch(int kind, const ProductArgs& a, cudaStream_t stream) {
 template <typename T>
 void Sum(const RoutedSumArgs& a, cudaStream_t stream) {
   if (a.tokens == 0 || a.width == 0) return;
-  const int64_t chunks = (a.width + 255) / 256;
-  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>((a.tokens * chunks + 7) / 8, 1 << 20));
+  const dim3 blocks(static_cast<unsigned>(std::min<int64_t>((a.tokens + 7) / 8, 1 << 20)),
+                    static_cast<unsigned>((a.width + 255) / 256));   // a width is at most 2^23
   const bool vector = a.width % 8 == 0 && a.y_stride % 8 == 0 && a.out_stride % 8 == 0 &&
                       reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
-  if (vector) RoutedSum<T, true><<<blocks, 256, 0, stream>>>(a, chunks);
-  else RoutedSum<T, false><<<blocks, 256, 0, stream>>>(a, chunks);
+  if (vector) RoutedSum<T, true><<<blocks, 256, 0, stream>>>(a);
+  else RoutedSum<T, false><<<blocks, 256, 0, stream>>>(a);
   Check(cudaGetLastError(), "routed sum launch");
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
 }

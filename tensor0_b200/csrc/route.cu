@@ -59,6 +59,17 @@ __device__ __forceinline__ double WarpSum(double v) {
   return v;
 }
 
+// Sum over lanes 0 to top_k - 1 (the others hold 0), valid in those lanes.
+__device__ __forceinline__ float ChosenSum(float v, int top_k) {
+  if (top_k > 8) {
+    v += __shfl_xor_sync(kFull, v, 16);
+    v += __shfl_xor_sync(kFull, v, 8);
+  }
+#pragma unroll
+  for (int d = 4; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+  return v;
+}
+
 // The lane's experts of a token; `vector`: as one access (rows start on
 // multiples of it).
 template <typename T, int V>
@@ -191,10 +202,11 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
     float top = 0.0f, total = 1.0f;
     bool nan = false;
     if (a.softmax != 0) {
-      top = Largest<V>(x);
 #pragma unroll
       for (int j = 0; j < V; ++j) nan = nan || x[j] != x[j];
       nan = __any_sync(kFull, nan);
+      // Where the first pick is the largest logit, it is known from there.
+      if (!kByLogit || a.renormalize == 0 || a.groups > 1) top = Largest<V>(x);
     }
     if constexpr (kByLogit) {
       if (a.softmax != 0 && (a.renormalize == 0 || a.groups > 1)) {
@@ -260,6 +272,7 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
       for (int j = 1; j < V; ++j) best = max(best, key[j]);
       const uint32_t largest = __reduce_max_sync(kFull, best);
       if (largest == 0u) break;
+      if (kByLogit && n == 0 && a.groups == 1 && a.renormalize != 0) top = Unordered(largest);
       const int winner = __ffs(__ballot_sync(kFull, best == largest)) - 1;
       int at = V - 1;
 #pragma unroll
@@ -278,10 +291,11 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
     if (mine >= 0) {
       const float logit = kByLogit ? Unordered(mine_key)
                                    : ToFloat(static_cast<const T*>(a.logits)[t * a.logit_stride + mine]);
-      score = a.softmax != 0 ? __fdiv_rn(expf(logit - top), total) : __frcp_rn(1.0f + expf(-logit));
+      // The weights need no more than the divisions' two units in the last place.
+      score = a.softmax != 0 ? __fdividef(expf(logit - top), total) : __fdividef(1.0f, 1.0f + expf(-logit));
       if (nan) score = __uint_as_float(0x7fc00000u);
     }
-    if (a.renormalize != 0) score = __fdiv_rn(score, WarpSum(score) + 1e-20f);
+    if (a.renormalize != 0) score = __fdividef(score, ChosenSum(score, a.top_k) + 1e-20f);
     if (lane < a.top_k) {
       chosen[lane] = mine;
       weights[lane] = mine < 0 ? 0.0f : score * a.scale;
@@ -476,68 +490,67 @@ __global__ void __launch_bounds__(kPlaceThreads) RoutePlace(RouteArgs a, int64_t
 //   renormalised: g <- (g - sum(g p) / total) / total, total = sum p + 1e-20
 //   softmax: dx_j = s_j (ds_j - sum(g p)),  ds the scattered g
 //   sigmoid: dx_j = ds_j s_j (1 - s_j)
-// Memory bound: reads and writes each logit once; the scores are recomputed.
-template <typename T, int V>
+// Reads and writes each logit once; the scores are recomputed, with the fast
+// exponential (about 1e-6 of a score far below the largest, less near it).  A
+// warp has one token: instructions bound it, and a loop's cost more than launching.
+template <typename T, int V, bool kSoftmax>
 __global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs a, bool vector) {
-  extern __shared__ float scattered[];   // one row of experts per warp: ds, zero between tokens
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int64_t step = int64_t{gridDim.x} * warps;
-  float* ds = scattered + warp * (32 * V);
+  __shared__ __align__(16) float scattered[kRouteThreads / 32][32 * V];   // ds
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t = static_cast<int>(blockIdx.x) * (kRouteThreads / 32) + warp;   // tokens * top_k is below 2^31
+  if (t >= static_cast<int>(a.tokens)) return;
+  const T* row = static_cast<const T*>(a.logits) + int64_t{t} * static_cast<int>(a.logit_stride);
+  int mine = -1;
+  float g = 0.0f, logit = -INFINITY, d[V];
+  if (lane < a.top_k) {
+    mine = a.chosen[t * a.top_k + lane];
+    g = a.weights_grad[t * a.top_k + lane] * a.scale;
+  }
+  float* ds = scattered[warp];
 #pragma unroll
-  for (int j = 0; j < V; ++j) ds[j * 32 + lane] = 0.0f;
-  __syncwarp();
-  for (int64_t t = int64_t{blockIdx.x} * warps + warp; t < a.tokens; t += step) {
-    T* out = static_cast<T*>(a.logits_grad) + t * a.experts;
-    const T* row = static_cast<const T*>(a.logits) + t * a.logit_stride;
-    const int mine = lane < a.top_k ? a.chosen[t * a.top_k + lane] : -1;
-    const bool found = mine >= 0 && mine < a.experts;
-    float g = found ? a.weights_grad[t * a.top_k + lane] * a.scale : 0.0f;
-    float d[V];
-    if (__ballot_sync(kFull, found) == 0u) {   // no expert: the logits may hold anything
+  for (int j = 0; j < V; ++j) ds[j * 32 + lane] = d[j] = 0.0f;
+  const bool found = mine >= 0 && mine < a.experts;
+  if (__any_sync(kFull, found)) {   // otherwise the logits may hold anything
+    if (found) logit = ToFloat(row[mine]);
+    if (!found) g = 0.0f;
+    float x[V], p;
+    if constexpr (kSoftmax) {
+      LoadLogits<T, V>(row, a.experts, lane, vector, x);   // -inf past the last expert
+      const float top = Largest<V>(x);
+      float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = 0.0f;
+      for (int j = 0; j < V; ++j) {
+        x[j] = __expf(x[j] - top);
+        sum += x[j];
+      }
+      const float inverse = __fdividef(1.0f, WarpSum(sum));
+      p = __expf(logit - top) * inverse;
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j] *= inverse;
     } else {
-      float x[V], top = 0.0f, inverse = 1.0f, p = 0.0f;
-      LoadLogits<T, V>(row, a.experts, lane, vector, x);
-      const float logit = found ? ToFloat(row[mine]) : 0.0f;
-      if (a.softmax != 0) {
-        top = Largest<V>(x);
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          x[j] = lane * V + j < a.experts ? expf(x[j] - top) : 0.0f;
-          sum += x[j];
-        }
-        inverse = __frcp_rn(WarpSum(sum));
-        if (found) p = expf(logit - top) * inverse;
-      } else if (found) {
-        p = __frcp_rn(1.0f + expf(-logit));
-      }
-      if (a.renormalize != 0) {
-        const float total = __frcp_rn(WarpSum(p) + 1e-20f);
-        const float mean = WarpSum(g * (p * total));
-        g = found ? (g - mean) * total : 0.0f;
-      }
+      p = __fdividef(1.0f, 1.0f + __expf(-logit));
+    }
+    if (a.renormalize != 0) {
+      const float total = __fdividef(1.0f, ChosenSum(p, a.top_k) + 1e-20f);
+      const float mean = ChosenSum(g * (p * total), a.top_k);
+      g = found ? (g - mean) * total : 0.0f;
+    }
+    if constexpr (kSoftmax) {
+      const float inner = __shfl_sync(kFull, ChosenSum(g * p, a.top_k), 0);
+      __syncwarp();
       if (found) ds[mine] = g;
       __syncwarp();
-      if (a.softmax != 0) {
-        const float inner = WarpSum(g * p);
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = x[j] * inverse * (ds[lane * V + j] - inner);
-      } else {
+      for (int j = 0; j < V; ++j) d[j] = x[j] * (ds[lane * V + j] - inner);
+    } else {
+      __syncwarp();
+      if (found) ds[mine] = g * p * (1.0f - p);
+      __syncwarp();
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float g_j = ds[lane * V + j];
-          const float s = __frcp_rn(1.0f + expf(-x[j]));
-          d[j] = g_j != 0.0f ? g_j * s * (1.0f - s) : 0.0f;
-        }
-      }
-      __syncwarp();
-      if (found) ds[mine] = 0.0f;
-      __syncwarp();
+      for (int j = 0; j < V; ++j) d[j] = ds[lane * V + j];
     }
-    StoreValues<T, V>(out, a.experts, lane, vector, d);
   }
+  StoreValues<T, V>(static_cast<T*>(a.logits_grad) + int64_t{t} * a.experts, a.experts, lane, vector, d);
 }
 
 // Up to this many tokens one block does the whole call.
@@ -546,7 +559,7 @@ constexpr int64_t kOneBlockTokens = 64;
 // Counting blocks: enough to fill the device with warps, each with its eight
 // warps' tokens at least.
 int64_t TokensPerBlock(int64_t tokens) {
-  const int64_t blocks = int64_t{RoutedSmCount()} * 4;
+  const int64_t blocks = int64_t{RoutedSmCount()} * 8;
   return std::max<int64_t>(8, ((tokens + blocks - 1) / blocks + 7) / 8 * 8);
 }
 
@@ -592,9 +605,10 @@ void Route(const RouteArgs& a, cudaStream_t stream) {
 
 template <typename T, int V>
 void Backward(const RouteBackwardArgs& a, cudaStream_t stream) {
-  const int64_t blocks = std::min<int64_t>((a.tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32), 1 << 20);
+  const unsigned blocks = static_cast<unsigned>((a.tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32));
   const bool vector = VectorLogits<T, V>(a.logits, a.logit_stride) && VectorLogits<T, V>(a.logits_grad, a.experts);
-  RouteBackward<T, V><<<static_cast<unsigned>(blocks), kRouteThreads, kRouteThreads * V * sizeof(float), stream>>>(a, vector);
+  if (a.softmax != 0) RouteBackward<T, V, true><<<blocks, kRouteThreads, 0, stream>>>(a, vector);
+  else RouteBackward<T, V, false><<<blocks, kRouteThreads, 0, stream>>>(a, vector);
   Check(cudaGetLastError(), "router gradient launch");
   g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
 }
