@@ -187,18 +187,21 @@ __device__ __forceinline__ float GroupScore(const float (&c)[V], int experts, in
 template <typename T, int V, bool kByLogit>
 __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, int64_t end, float* values, bool vector) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  for (int64_t t = begin + warp; t < end; t += warps) {
-    int32_t* chosen = a.chosen + t * a.top_k;
-    float* weights = a.weights + t * a.top_k;
+  // tokens * top_k and a row stride are below 2^31: 32-bit indices, which cost a
+  // tenth of the instructions less than 64-bit ones.
+  const int stride = static_cast<int>(a.logit_stride), last = static_cast<int>(end);
+  for (int t = static_cast<int>(begin) + warp; t < last; t += warps) {
+    const int entry = t * a.top_k + lane;
     if (a.mask != nullptr && a.mask[t] == 0) {   // its logits may hold anything
       if (lane < a.top_k) {
-        chosen[lane] = -1;
-        weights[lane] = 0.0f;
+        a.chosen[entry] = -1;
+        a.weights[entry] = 0.0f;
       }
       continue;
     }
+    const T* row = static_cast<const T*>(a.logits) + int64_t{t} * stride;
     float x[V], c[V];   // c: what the choice goes by
-    LoadLogits<T, V>(static_cast<const T*>(a.logits) + t * a.logit_stride, a.experts, lane, vector, x);
+    LoadLogits<T, V>(row, a.experts, lane, vector, x);
     float top = 0.0f, total = 1.0f;
     bool nan = false;
     if (a.softmax != 0) {
@@ -266,13 +269,13 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
     }
     int mine = -1;
     uint32_t mine_key = 0;
+#pragma unroll 1
     for (int n = 0; n < a.top_k; ++n) {
       uint32_t best = key[0];
 #pragma unroll
       for (int j = 1; j < V; ++j) best = max(best, key[j]);
       const uint32_t largest = __reduce_max_sync(kFull, best);
       if (largest == 0u) break;
-      if (kByLogit && n == 0 && a.groups == 1 && a.renormalize != 0) top = Unordered(largest);
       const int winner = __ffs(__ballot_sync(kFull, best == largest)) - 1;
       int at = V - 1;
 #pragma unroll
@@ -288,17 +291,17 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
       }
     }
     float score = 0.0f;
+    if (kByLogit && a.groups == 1 && a.renormalize != 0) top = Unordered(__shfl_sync(kFull, mine_key, 0));
     if (mine >= 0) {
-      const float logit = kByLogit ? Unordered(mine_key)
-                                   : ToFloat(static_cast<const T*>(a.logits)[t * a.logit_stride + mine]);
+      const float logit = kByLogit ? Unordered(mine_key) : ToFloat(row[mine]);
       // The weights need no more than the divisions' two units in the last place.
       score = a.softmax != 0 ? __fdividef(expf(logit - top), total) : __fdividef(1.0f, 1.0f + expf(-logit));
       if (nan) score = __uint_as_float(0x7fc00000u);
     }
     if (a.renormalize != 0) score = __fdividef(score, ChosenSum(score, a.top_k) + 1e-20f);
     if (lane < a.top_k) {
-      chosen[lane] = mine;
-      weights[lane] = mine < 0 ? 0.0f : score * a.scale;
+      a.chosen[entry] = mine;
+      a.weights[entry] = mine < 0 ? 0.0f : score * a.scale;
     }
   }
 }
