@@ -421,37 +421,47 @@ __global__ void __launch_bounds__(kRouteThreads) RouteSelect(RouteArgs a, int64_
 }
 
 // Each block's counts become the counts of the blocks before it; the totals go
-// in the row after the last block's.  A block has 32 experts, a warp a run of
-// the counting blocks.
-constexpr int kScanWarps = 32;
-__global__ void __launch_bounds__(kScanWarps * 32) RouteScan(RouteArgs a, int blocks) {
-  __shared__ int sums[kScanWarps][33];
+// in the row after the last block's.  A block has 8 experts (a 32-byte sector of
+// every row of counts), a thread a run of one expert's counts.
+constexpr int kScanThreads = 1024, kScanExperts = 8;
+__global__ void __launch_bounds__(kScanThreads) RouteScan(RouteArgs a, int blocks) {
+  constexpr int kRuns = kScanThreads / kScanExperts, kWarps = kScanThreads / 32;
+  __shared__ int sums[kWarps][kScanExperts];
   LetNextStart();
   WaitForPrevious();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
-  const int run = (blocks + kScanWarps - 1) / kScanWarps, from = warp * run, to = min(blocks, from + run);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int column = lane % kScanExperts, e = blockIdx.x * kScanExperts + column;
+  const int run = (blocks + kRuns - 1) / kRuns, from = threadIdx.x / kScanExperts * run, to = min(blocks, from + run);
+  int32_t* cells = a.counts + e;
   int sum = 0;
   if (e < a.experts) {
 #pragma unroll 8
-    for (int b = from; b < to; ++b) sum += a.counts[b * int64_t{a.experts} + e];
+    for (int b = from; b < to; ++b) sum += cells[b * int64_t{a.experts}];
   }
-  sums[warp][lane] = sum;
-  __syncthreads();
-  if (e >= a.experts) return;
-  int before = 0, all = 0;
+  int before = sum;   // of the runs before this one in the warp, and this one
 #pragma unroll
-  for (int w = 0; w < kScanWarps; ++w) {
-    before += w < warp ? sums[w][lane] : 0;
-    all += sums[w][lane];
+  for (int d = kScanExperts; d < 32; d *= 2) {
+    const int other = __shfl_up_sync(kFull, before, d);
+    if (lane >= d) before += other;
   }
+  if (lane >= 32 - kScanExperts) sums[warp][column] = before;
+  before -= sum;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int value = sums[w][column];
+    before += w < warp ? value : 0;
+    all += value;
+  }
+  if (e >= a.experts) return;
 #pragma unroll 8
   for (int b = from; b < to; ++b) {
-    int32_t* cell = a.counts + b * int64_t{a.experts} + e;
-    const int count = *cell;
-    *cell = before;
+    const int count = cells[b * int64_t{a.experts}];
+    cells[b * int64_t{a.experts}] = before;
     before += count;
   }
-  if (warp == 0) a.counts[blocks * int64_t{a.experts} + e] = all;
+  if (threadIdx.x < kScanExperts) cells[blocks * int64_t{a.experts}] = all;
 }
 
 constexpr int kPlaceThreads = 128;
@@ -600,7 +610,7 @@ void Route(const RouteArgs& a, cudaStream_t stream) {
   const std::size_t select = (bins + (a.groups > 1 ? kRouteThreads / 32 * bins : 0)) * sizeof(int);
   RouteSelect<T, V, kByLogit><<<blocks, kRouteThreads, select, stream>>>(a, per_block, vector);
   Check(cudaGetLastError(), "router launch");
-  LaunchAfter(RouteScan, static_cast<unsigned>((a.experts + 31) / 32), kScanWarps * 32, 0, stream, a,
+  LaunchAfter(RouteScan, static_cast<unsigned>((a.experts + kScanExperts - 1) / kScanExperts), kScanThreads, 0, stream, a,
               static_cast<int>(blocks));
   LaunchAfter(RoutePlace, blocks, kPlaceThreads, (1 + kPlaceThreads / 32) * bins * sizeof(int), stream, a, per_block);
   g_kernel_launches.fetch_add(3, std::memory_order_relaxed);
