@@ -190,6 +190,7 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
   // tokens * top_k and a row stride are below 2^31: 32-bit indices, which cost a
   // tenth of the instructions less than 64-bit ones.
   const int stride = static_cast<int>(a.logit_stride), last = static_cast<int>(end);
+  const bool bias_vector = reinterpret_cast<uintptr_t>(a.bias) % (V * 4 < 16 ? V * 4 : 16) == 0;
   for (int t = static_cast<int>(begin) + warp; t < last; t += warps) {
     const int entry = t * a.top_k + lane;
     if (a.mask != nullptr && a.mask[t] == 0) {   // its logits may hold anything
@@ -240,8 +241,10 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
         for (int j = 0; j < V; ++j) c[j] = __frcp_rn(1.0f + expf(-x[j]));
       }
       if (a.bias != nullptr) {
+        float b[V];
+        LoadLogits<float, V>(a.bias, a.experts, lane, bias_vector, b);   // -inf past the last expert
 #pragma unroll
-        for (int j = 0; j < V; ++j) c[j] += lane * V + j < a.experts ? a.bias[lane * V + j] : 0.0f;
+        for (int j = 0; j < V; ++j) c[j] += b[j];
       }
     }
     uint32_t key[V];
@@ -260,11 +263,18 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
         kept |= 1u << winner;
         if (lane == winner) group_key = 0u;
       }
-      const int size = a.experts / a.groups;
+      // The lane's experts by their group, with one division.
+      const int size = a.experts / a.groups, group = lane * V / size;
+      int left = (group + 1) * size - lane * V;   // experts of this group from here on
+      uint32_t bits = group < 32 ? kept >> group : 0u;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int e = lane * V + j;
-        if (e < a.experts && ((kept >> (e / size)) & 1u) == 0u) key[j] = 0u;
+        if (left == 0) {
+          bits >>= 1;
+          left = size;
+        }
+        --left;
+        if ((bits & 1u) == 0u) key[j] = 0u;
       }
     }
     int mine = -1;
