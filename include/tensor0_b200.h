@@ -342,7 +342,8 @@ int t0b_routed_sum(int32_t dtype, int64_t tokens, int32_t top_k, int32_t width, 
  * group 32, 64 or 128 neighbours of one half (scale = max|h| / 127, codes rounded
  * half to even; a group with a NaN or infinity loads as NaN; one below 2^-100 as
  * zeros).  w = weights[rows[p]] with a routing, else 1 (weights, row_entries and
- * offsets all NULL); rows without an expert are not read and give zeros.
+ * offsets all NULL); rows without an expert are not read and give zeros.  codes
+ * and scales both NULL: the activation alone.
  */
 int t0b_gated_save(int32_t dtype, int64_t row_count, int32_t width, int32_t group, const void* h, int64_t h_stride,
                    const float* weights, const int32_t* row_entries, const int32_t* offsets, int32_t experts,

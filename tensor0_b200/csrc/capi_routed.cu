@@ -311,8 +311,10 @@ int t0b_gated_save(int32_t dtype, int64_t row_count, int32_t width, int32_t grou
     const int64_t groups = (int64_t{width} + group - 1) / group;
     const uint64_t h_bytes = Operand(h, row_count, int64_t{2} * width, h_stride, item, "activation input");
     const uint64_t a_bytes = Packed(a, row_count, width, item, "activation");
-    const uint64_t code_bytes = Packed(codes, row_count, int64_t{2} * width, 1, "checkpoint code");
-    const uint64_t scale_bytes = Packed(scales, row_count, 2 * groups, 4, "checkpoint scale");
+    Require((codes == nullptr) == (scales == nullptr), "a checkpoint is its codes and its scales");
+    const int64_t kept = codes != nullptr ? row_count : 0;
+    const uint64_t code_bytes = Packed(codes, kept, int64_t{2} * width, 1, "checkpoint code");
+    const uint64_t scale_bytes = Packed(scales, kept, 2 * groups, 4, "checkpoint scale");
     Separate({{a, a_bytes}, {codes, code_bytes}, {scales, scale_bytes}},
              {{h, h_bytes}, {weights, entry_bytes}, {row_entries, entry_bytes}});
     if (row_count == 0) return;

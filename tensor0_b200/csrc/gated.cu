@@ -161,6 +161,7 @@ __global__ void __launch_bounds__(kGatedThreads) GatedSave(GatedArgs a) {
         for (int i = 0; i < 8; ++i) out[i] = 0.0f;
       }
       Store8<T, Vector>(out_row + column, count, out);
+      if (a.codes == nullptr) continue;   // the activation alone
       StoreCodes<Vector>(g, count, lanes, lane, code_row + column, scale_row + (column >> shift));
       StoreCodes<Vector>(u, count, lanes, lane, code_row + a.width + column, scale_row + groups + (column >> shift));
     }

@@ -333,6 +333,19 @@ def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 
     return a, kept
 
 
+def gated(h: torch.Tensor, *, routing: Routing | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``gated_save``'s activation alone, for a pass that has no backward one."""
+    if h.dim() != 2 or h.shape[1] % 2 or h.shape[1] == 0:
+        raise ValueError("h must be [rows, 2 * width]")
+    rows, width = h.shape[0], h.shape[1] // 2
+    device = _device(h, *(() if routing is None else (routing.weights, routing.rows, routing.offsets)))
+    code = _code(_HALF, h, "gated activations")
+    address, stride = _rows(h, rows, 2 * width, "h")
+    out, result = _output(h, out, (rows, width))
+    _gated_save(device, code, rows, width, 128, address, stride, *_row_weights(routing, rows), result, None, None)
+    return out
+
+
 def _checkpoint(checkpoint: Checkpoint) -> tuple[int, int, int, int]:
     """(rows, width, codes, scales) of a checkpoint whose arrays agree."""
     codes, scales, group = checkpoint

@@ -499,6 +499,15 @@ def test_gated(tokens, top_k, width, group, with_routing, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("with_routing", [False, True])
+def test_gated_without_a_checkpoint(with_routing):
+    _, r = make_routing(70, 8, 3, 14, absent=0.2)
+    h = torch.randn(210, 2 * 136).bfloat16().cuda()
+    a, _ = routed.gated_save(h, routing=r if with_routing else None)
+    assert torch.equal(routed.gated(h, routing=r if with_routing else None), a)
+
+
+@gpu
 def test_gated_gradient_against_differences():
     """The gradient against central differences of the plain activation at the checkpoint's values."""
     width, group = 40, 32
@@ -653,6 +662,7 @@ def test_product_refusals(change, message):
     ("t0b_gated_save", (10, 4, 8, 32, A, 15, None, None, None, 0, B, C, D), "stride"),
     ("t0b_gated_save", (10, 4, 8, 32, A, 16, E, None, None, 2, B, C, D), "routing"),
     ("t0b_gated_save", (10, 4, 8, 32, A, 16, None, None, None, 0, A, C, D), "overlap"),
+    ("t0b_gated_save", (10, 4, 8, 32, A, 16, None, None, None, 0, B, C, None), "codes and its scales"),
     ("t0b_gated_backward", (10, 4, 8, 32, A, B, C, 8, None, None, None, 0, D, D, E), "overlap"),
     ("t0b_checkpoint_load", (12, 4, 8, 32, A, B, C), "F32, F16 or BF16"),
     ("t0b_routed_matvec4", (10, 8, 2, 2, 48, 32, 32, 1, A, 4, 48, B, C, D, E, F), "divide"),
