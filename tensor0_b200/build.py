@@ -5,6 +5,9 @@ Compiles every CUDA / C++ source under ``csrc/`` with nvcc for
 runtime, so the library loads on hosts without a GPU driver (the CPU test
 suite checks its exported symbols there).
 
+``build_binding()`` compiles the Python binding of the routed operators
+(``_lib/_routed.so``, source ``binding/routed.cpp``) against the installed torch.
+
 ``build_xla()`` links the XLA FFI handler library
 (``_lib/libtensor0_b200_xla.so``, source ``xla/handlers.cu``) on top of it.
 It needs the XLA FFI headers (``xla/ffi/api/ffi.h``): from
@@ -19,6 +22,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -27,6 +31,8 @@ CSRC = PACKAGE / "csrc"
 OUT = PACKAGE / "_lib"
 BUILD = PACKAGE / "_build"
 LIBRARY = OUT / "libtensor0_b200.so"
+BINDING_SOURCE = PACKAGE / "binding" / "routed.cpp"
+BINDING = OUT / "_routed.so"
 XLA_SOURCE = PACKAGE / "xla" / "handlers.cu"
 XLA_LIBRARY = OUT / "libtensor0_b200_xla.so"
 
@@ -81,6 +87,29 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     return LIBRARY
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile the routed operators' Python binding on top of the library."""
+    import torch   # its headers and libraries
+
+    library = build(verbose=verbose)
+    inputs = [BINDING_SOURCE, PACKAGE.parent / "include" / "tensor0_b200.h", Path(__file__)]
+    if _stale(BINDING, inputs):
+        home = Path(torch.__file__).resolve().parent
+        cuda = Path(nvcc()).resolve().parents[1]
+        command = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+                   f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                   "-I", str(PACKAGE.parent / "include"), "-isystem", sysconfig.get_paths()["include"],
+                   "-isystem", str(home / "include"),
+                   "-isystem", str(home / "include" / "torch" / "csrc" / "api" / "include"),
+                   "-isystem", str(cuda / "include"), str(BINDING_SOURCE), "-o", str(BINDING),
+                   "-L", str(home / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+                   "-L", str(OUT), f"-l:{library.name}", "-Wl,-rpath,$ORIGIN"]
+        if verbose:
+            print(" ".join(command), flush=True)
+        subprocess.run(command, check=True)
+    return BINDING
+
+
 def xla_ffi_include() -> Path | None:
     """The directory holding ``xla/ffi/api/ffi.h``, or None."""
     candidates = []
@@ -120,4 +149,5 @@ def build_xla(verbose: bool = False) -> Path | None:
 
 if __name__ == "__main__":
     print(build(verbose=True))
+    print(build_binding(verbose=True))
     print(build_xla(verbose=True))

@@ -22,17 +22,38 @@ latency-bound step allocates nothing.
 
 from __future__ import annotations
 
-import threading
+import importlib.machinery
+import importlib.util
 from typing import NamedTuple
 
 import torch
 
 from . import _native
+from . import build as _build
 
 _HALF = {torch.float16: _native.F16, torch.bfloat16: _native.BF16}
 _FLOAT = {torch.float32: _native.F32, **_HALF}
-_SCORE = {"softmax": 0, "sigmoid": 1}
-_INT, _REAL = torch.int32, torch.float32
+
+
+class _Binding:
+    """The compiled binding (``binding/routed.cpp``), loaded at its first use.
+
+    It checks the tensors' types, shapes, strides and devices, allocates the results and calls the C entry points.
+    """
+
+    def __getattr__(self, name: str):
+        if not _build.BINDING.exists():
+            raise RuntimeError(f"tensor0_b200 binding not found at {_build.BINDING}; run "
+                               "tensor0_b200.build.build_binding() (there is no CPU fallback for the routed operators)")
+        _native.lib()
+        loader = importlib.machinery.ExtensionFileLoader("_routed", str(_build.BINDING))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_routed", loader))
+        loader.exec_module(module)
+        self.__dict__.update({key: value for key, value in vars(module).items() if not key.startswith("__")})
+        return self.__dict__[name]
+
+
+_routed = _Binding()
 
 
 class Routing(NamedTuple):
@@ -61,114 +82,12 @@ class Int4Weights(NamedTuple):
     group: int
 
 
-def _device(*tensors: torch.Tensor) -> int:
-    """Index of the CUDA device that holds all the tensors."""
-    index = tensors[0].get_device()   # -1 for host storage
-    for tensor in tensors:
-        if tensor.get_device() != index or not tensor.is_cuda:
-            if not tensor.is_cuda or not tensors[0].is_cuda:
-                raise ValueError("routed storage must be a CUDA tensor (there is no CPU fallback)")
-            raise ValueError("routed operands must be on one device")
-    return index
-
-
-def _packed(tensor: torch.Tensor, shape: tuple, dtype: torch.dtype, what: str) -> int:
-    if tensor.dtype is dtype and tensor.shape == shape and tensor.is_contiguous():
-        return tensor.data_ptr()
-    raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {list(shape)}, got {tensor.dtype} "
-                     f"{list(tensor.shape)} with strides {list(tensor.stride())}")
-
-
-def _output(like: torch.Tensor, out: torch.Tensor | None, shape: tuple) -> tuple[torch.Tensor, int]:
-    """The result of an operator and its address: new, or ``out`` if that fits."""
-    if out is None:
-        out = like.new_empty(shape)
-        return out, out.data_ptr()
-    _device(like, out)
-    return out, _packed(out, shape, like.dtype, "out")
-
-
-def _rows(x: torch.Tensor, rows: int, width: int, what: str, gather: bool = False) -> tuple[int, int]:
-    """(address, row stride) of a matrix of that shape whose rows are contiguous."""
-    if x.shape != (rows, width):
-        kind = "token" if gather else "expert-ordered"
-        raise ValueError(f"{what} must be [{rows}, {width}] ({kind} rows), got {list(x.shape)}")
-    stride, step = x.stride()
-    if step != 1 and width > 1:
-        raise ValueError(f"{what} must have contiguous rows")
-    return x.data_ptr(), stride if rows > 1 or stride > width else width
-
-
-def _code(table: dict, tensor: torch.Tensor, what: str) -> int:
-    code = table.get(tensor.dtype)
-    if code is None:
-        raise ValueError(f"{what} must be {' or '.join(str(t)[6:] for t in table)}, got {tensor.dtype}")
-    return code
-
-
-class _Entry:
-    """A C entry point: called with its arguments up to the stream, on the device's current stream.
-
-    Small operators take less time than their checks, so a call costs as little as it can: the function is looked up
-    once, a thread keeps its error buffer, and the stream is asked for its handle alone.
-    """
-
-    local = threading.local()
-
-    def __init__(self, name: str):
-        self.name = name
-        self.function = None
-
-    def __call__(self, device: int, *arguments) -> None:
-        function = self.function
-        if function is None:
-            function = self.function = getattr(_native.lib(), self.name)
-        try:
-            err = self.local.err
-        except AttributeError:
-            err = self.local.err = _native.error_buffer()
-        stream = torch._C._cuda_getCurrentRawStream(device)
-        if torch._C._cuda_getDevice() == device:
-            status = function(*arguments, stream, err, 512)
-        else:
-            with torch.cuda.device(device):
-                status = function(*arguments, stream, err, 512)
-        if status != 0:
-            _native.check(status, err)
-
-
-_route, _route_backward = _Entry("t0b_route"), _Entry("t0b_route_backward")
-_product, _weight_grad, _sum = _Entry("t0b_routed_product"), _Entry("t0b_routed_weight_grad"), _Entry("t0b_routed_sum")
-_gated_save, _gated_backward = _Entry("t0b_gated_save"), _Entry("t0b_gated_backward")
-_checkpoint_load, _matvec4 = _Entry("t0b_checkpoint_load"), _Entry("t0b_routed_matvec4")
-
-
-def _entries(routing: Routing) -> tuple[int, int, int, int, int]:
-    """(tokens, top_k, experts, rows, offsets) of a routing whose arrays agree; the last two are addresses."""
-    chosen, _, rows, _, offsets = routing
-    if chosen.dim() != 2:
-        raise ValueError("routing experts must be [tokens, top_k]")
-    tokens, top_k = chosen.shape
-    experts = offsets.numel() - 1
-    if experts < 1:
-        raise ValueError("routing offsets must be [experts + 1]")
-    return (tokens, top_k, experts, _packed(rows, (tokens * top_k,), _INT, "routing rows"),
-            _packed(offsets, (experts + 1,), _INT, "routing offsets"))
-
-
 def empty_routing(tokens: int, top_k: int, experts: int, device="cuda") -> Routing:
     """Uninitialised buffers for ``route(..., out=...)``."""
     def ints(*shape):
         return torch.empty(shape, dtype=torch.int32, device=device)
     return Routing(ints(tokens, top_k), torch.empty(tokens, top_k, dtype=torch.float32, device=device),
                    ints(tokens * top_k), ints(tokens, top_k), ints(experts + 1))
-
-
-def _score(score: str) -> int:
-    code = _SCORE.get(score)
-    if code is None:
-        raise ValueError("score must be 'softmax' or 'sigmoid'")
-    return code
 
 
 def route(logits: torch.Tensor, top_k: int, *, groups: int = 1, top_groups: int | None = None, group_best: int = 1,
@@ -183,29 +102,11 @@ def route(logits: torch.Tensor, top_k: int, *, groups: int = 1, top_groups: int 
     (``group_best`` 1) or sum of the two best (2) stay.  ``renormalize`` divides the chosen scores by their sum.
     ``mask`` (bool [tokens]): tokens that are False take no expert, whatever their logits hold.
     """
-    if logits.dim() != 2:
-        raise ValueError("logits must be [tokens, experts]")
-    tokens, experts = logits.shape
-    device = _device(logits, *[t for t in (bias, mask) if t is not None])
-    code = _code(_FLOAT, logits, "logits")
-    address, stride = _rows(logits, tokens, experts, "logits")
-    bias_pointer = None if bias is None else _packed(bias, (experts,), _REAL, "bias")
-    mask_pointer = None if mask is None else _packed(mask, (tokens,), torch.bool, "mask")
     if out is None:
-        out = empty_routing(tokens, top_k, experts, logits.device)
-    else:
-        _device(logits, *out)
-    chosen, weights, rows, positions, offsets = out
-    entry = (tokens, top_k)
-    size = _native.lib().t0b_route_workspace(tokens, experts)
-    workspace = logits.new_empty(size, dtype=torch.uint8).data_ptr() if size else None
-    _route(device, code, tokens, experts, top_k, groups, groups if top_groups is None else top_groups, group_best,
-           _score(score), int(renormalize), scale, address, stride, bias_pointer, mask_pointer,
-           _packed(chosen, entry, _INT, "routing experts"), _packed(weights, entry, _REAL, "routing weights"),
-           _packed(rows, (tokens * top_k,), _INT, "routing rows"),
-           _packed(positions, entry, _INT, "routing positions"),
-           _packed(offsets, (experts + 1,), _INT, "routing offsets"), workspace, size)
-    return out
+        if logits.dim() != 2:
+            raise ValueError("logits must be [tokens, experts]")
+        out = empty_routing(logits.shape[0], max(top_k, 0), logits.shape[1], logits.device)
+    return _routed.route(logits, top_k, groups, top_groups, group_best, score, renormalize, scale, bias, mask, out)
 
 
 def route_backward(logits: torch.Tensor, routing: Routing, weights_grad: torch.Tensor, *, score: str = "softmax",
@@ -215,19 +116,7 @@ def route_backward(logits: torch.Tensor, routing: Routing, weights_grad: torch.T
     The choice of experts is piecewise constant and the bias enters it only, so neither has a gradient.  Tokens
     without an expert get zeros, whatever their logits hold.
     """
-    if logits.dim() != 2:
-        raise ValueError("logits must be [tokens, experts]")
-    tokens, experts = logits.shape
-    device = _device(logits, routing.experts, weights_grad)
-    code = _code(_FLOAT, logits, "logits")
-    address, stride = _rows(logits, tokens, experts, "logits")
-    top_k = routing.experts.shape[-1]
-    chosen = _packed(routing.experts, (tokens, top_k), _INT, "routing experts")
-    grad = _packed(weights_grad, (tokens, top_k), _REAL, "weights_grad")
-    out, result = _output(logits, out, (tokens, experts))
-    _route_backward(device, code, tokens, experts, top_k, _score(score), int(renormalize), scale, address, stride,
-                    chosen, grad, result)
-    return out
+    return _routed.route_backward(logits, routing, weights_grad, score, renormalize, scale, out)
 
 
 def routed_matmul(x: torch.Tensor, w: torch.Tensor, routing: Routing, *, gather: bool = False,
@@ -237,20 +126,7 @@ def routed_matmul(x: torch.Tensor, w: torch.Tensor, routing: Routing, *, gather:
     ``w`` [experts, inner, outer], float16 or bfloat16 as ``x``.  ``x`` holds token rows with ``gather`` (row p reads
     its entry's token), else expert-ordered rows.  Summed in 32 bits, rounded once; rows without an expert are zero.
     """
-    tokens, top_k, experts, rows, offsets = _entries(routing)
-    device = _device(x, w, routing.rows, routing.offsets)
-    code = _code(_HALF, x, "product operands")
-    if w.dim() != 3 or w.shape[0] != experts:
-        raise ValueError(f"weights must be [{experts}, inner, outer]")
-    _, inner, outer = w.shape
-    entries = tokens * top_k
-    x_rows = tokens if gather else entries
-    weights = _packed(w, w.shape, x.dtype, "weights")
-    address, stride = _rows(x, x_rows, outer if transpose else inner, "x", gather)
-    out, result = _output(x, out, (entries, inner if transpose else outer))
-    _product(device, code, int(transpose), entries, experts, top_k, inner, outer, int(gather), address, x_rows, stride,
-             weights, rows, offsets, result)
-    return out
+    return _routed.routed_matmul(x, w, routing, gather, transpose, out)
 
 
 def routed_weight_grad(x: torch.Tensor, y_grad: torch.Tensor, routing: Routing, *, gather_x: bool = False,
@@ -260,45 +136,12 @@ def routed_weight_grad(x: torch.Tensor, y_grad: torch.Tensor, routing: Routing, 
     Either operand holds token rows (``gather_x``, ``gather_y``) or expert-ordered ones.  An expert without rows
     gets zeros.
     """
-    tokens, top_k, experts, rows, offsets = _entries(routing)
-    device = _device(x, y_grad, routing.rows, routing.offsets)
-    code = _code(_HALF, x, "product operands")
-    if y_grad.dtype != x.dtype:
-        raise ValueError("product operands must share a dtype")
-    inner, outer = x.shape[-1], y_grad.shape[-1]
-    entries = tokens * top_k
-    x_rows, y_rows = tokens if gather_x else entries, tokens if gather_y else entries
-    x_address, x_stride = _rows(x, x_rows, inner, "x", gather_x)
-    y_address, y_stride = _rows(y_grad, y_rows, outer, "y_grad", gather_y)
-    out, result = _output(x, out, (experts, inner, outer))
-    _weight_grad(device, code, entries, experts, top_k, inner, outer, int(gather_x), x_address, x_rows, x_stride,
-                 int(gather_y), y_address, y_rows, y_stride, rows, offsets, result)
-    return out
+    return _routed.routed_weight_grad(x, y_grad, routing, gather_x, gather_y, out)
 
 
 def routed_sum(y: torch.Tensor, routing: Routing, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """Each token's sum over its experts' rows: [tokens, width].  Also the gradient of gathering token rows."""
-    if routing.positions.dim() != 2:
-        raise ValueError("routing positions must be [tokens, top_k]")
-    tokens, top_k = routing.positions.shape
-    device = _device(y, routing.positions)
-    code = _code(_HALF, y, "sum operands")
-    positions = _packed(routing.positions, (tokens, top_k), _INT, "routing positions")
-    width = y.shape[-1]
-    address, stride = _rows(y, tokens * top_k, width, "y")
-    out, result = _output(y, out, (tokens, width))
-    _sum(device, code, tokens, top_k, width, address, stride, positions, result)
-    return out
-
-
-def _row_weights(routing: Routing | None, rows: int) -> tuple:
-    """(weights, rows, offsets, experts) arguments of the gated entry points."""
-    if routing is None:
-        return None, None, None, 0
-    tokens, top_k, experts, entries, offsets = _entries(routing)
-    if tokens * top_k != rows:
-        raise ValueError(f"the routing has {tokens * top_k} entries, the activation {rows} rows")
-    return _packed(routing.weights, (tokens, top_k), _REAL, "routing weights"), entries, offsets, experts
+    return _routed.routed_sum(y, routing, out)
 
 
 def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 128,
@@ -308,54 +151,16 @@ def gated_save(h: torch.Tensor, *, routing: Routing | None = None, group: int = 
     ``group`` (32, 64 or 128) neighbours of one half share a scale, their largest magnitude / 127.  A row's weight is
     its entry's in ``routing``, or 1 without one; with one, rows without an expert are not read and give zeros.
     """
-    if h.dim() != 2 or h.shape[1] % 2 or h.shape[1] == 0:
-        raise ValueError("h must be [rows, 2 * width]")
-    rows, width = h.shape[0], h.shape[1] // 2
-    device = _device(h, *(() if routing is None else (routing.weights, routing.rows, routing.offsets)))
-    code = _code(_HALF, h, "gated activations")
-    if group not in (32, 64, 128):
-        raise ValueError("checkpoint group must be 32, 64 or 128")
-    scales = 2 * -(-width // group)
-    address, stride = _rows(h, rows, 2 * width, "h")
-    if out is None:
-        a = h.new_empty((rows, width))
-        kept = Checkpoint(h.new_empty((rows, 2 * width), dtype=torch.int8),
-                          h.new_empty((rows, scales), dtype=torch.float32), group)
-    else:
-        a, kept = out
-        if kept.group != group:
-            raise ValueError("out's checkpoint has another group")
-        _device(h, a, kept.codes, kept.scales)
-    _gated_save(device, code, rows, width, group, address, stride, *_row_weights(routing, rows),
-                _packed(a, (rows, width), h.dtype, "out"),
-                _packed(kept.codes, (rows, 2 * width), torch.int8, "checkpoint codes"),
-                _packed(kept.scales, (rows, scales), _REAL, "checkpoint scales"))
-    return a, kept
+    a, kept = (None, (None, None, group)) if out is None else out
+    if kept[2] != group:
+        raise ValueError("out's checkpoint has another group")
+    a, codes, scales = _routed.gated_save(h, routing, group, a, kept[0], kept[1])
+    return a, Checkpoint(codes, scales, group)
 
 
 def gated(h: torch.Tensor, *, routing: Routing | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``gated_save``'s activation alone, for a pass that has no backward one."""
-    if h.dim() != 2 or h.shape[1] % 2 or h.shape[1] == 0:
-        raise ValueError("h must be [rows, 2 * width]")
-    rows, width = h.shape[0], h.shape[1] // 2
-    device = _device(h, *(() if routing is None else (routing.weights, routing.rows, routing.offsets)))
-    code = _code(_HALF, h, "gated activations")
-    address, stride = _rows(h, rows, 2 * width, "h")
-    out, result = _output(h, out, (rows, width))
-    _gated_save(device, code, rows, width, 128, address, stride, *_row_weights(routing, rows), result, None, None)
-    return out
-
-
-def _checkpoint(checkpoint: Checkpoint) -> tuple[int, int, int, int]:
-    """(rows, width, codes, scales) of a checkpoint whose arrays agree."""
-    codes, scales, group = checkpoint
-    if group not in (32, 64, 128):
-        raise ValueError("checkpoint group must be 32, 64 or 128")
-    if codes.dim() != 2 or codes.shape[1] % 2 or codes.shape[1] == 0:
-        raise ValueError("checkpoint codes must be [rows, 2 * width]")
-    rows, width = codes.shape[0], codes.shape[1] // 2
-    return (rows, width, _packed(codes, codes.shape, torch.int8, "checkpoint codes"),
-            _packed(scales, (rows, 2 * -(-width // group)), _REAL, "checkpoint scales"))
+    return _routed.gated_save(h, routing, None, out, None, None)
 
 
 def gated_backward(checkpoint: Checkpoint, a_grad: torch.Tensor, *, routing: Routing | None = None,
@@ -366,30 +171,14 @@ def gated_backward(checkpoint: Checkpoint, a_grad: torch.Tensor, *, routing: Rou
     ``weights_grad`` is the gradient of the routing's weights [tokens, top_k], or of a weight of 1 per row [rows]
     without a routing.
     """
-    rows, width, codes, scales = _checkpoint(checkpoint)
-    device = _device(a_grad, checkpoint.codes, checkpoint.scales,
-                     *(() if routing is None else (routing.weights, routing.rows, routing.offsets)))
-    code = _code(_HALF, a_grad, "gated activations")
-    address, stride = _rows(a_grad, rows, width, "a_grad")
-    weights = _row_weights(routing, rows)
-    h_grad = a_grad.new_empty((rows, 2 * width))
-    a = a_grad.new_empty((rows, width))
-    weights_grad = a_grad.new_empty((rows,) if routing is None else routing.weights.shape, dtype=torch.float32)
-    _gated_backward(device, code, rows, width, checkpoint.group, codes, scales, address, stride, *weights,
-                    h_grad.data_ptr(), a.data_ptr(), weights_grad.data_ptr())
-    return h_grad, a, weights_grad
+    return _routed.gated_backward(checkpoint, a_grad, routing)
 
 
 def checkpoint_load(checkpoint: Checkpoint, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values a checkpoint stands for, as float32, float16 or bfloat16."""
-    rows, width, codes, scales = _checkpoint(checkpoint)
-    device = _device(checkpoint.codes, checkpoint.scales)
     if dtype not in _FLOAT:
         raise ValueError("checkpoints load as float32, float16 or bfloat16")
-    values = checkpoint.codes.new_empty((rows, 2 * width), dtype=dtype)
-    _checkpoint_load(device, _FLOAT[dtype], rows, width, checkpoint.group, codes, scales,
-                     values.data_ptr())
-    return values
+    return _routed.checkpoint_load(checkpoint, _FLOAT[dtype])
 
 
 def pack_int4(w: torch.Tensor, group: int = 128) -> Int4Weights:
@@ -413,22 +202,5 @@ def routed_matvec(x: torch.Tensor, weights: Int4Weights, routing: Routing, *, ga
 
     Memory bound on the weights: each chosen expert's are read once however many rows it has.
     """
-    tokens, top_k, experts, rows, offsets = _entries(routing)
     codes, scales, group = weights
-    device = _device(x, codes, scales, routing.rows, routing.offsets)
-    code = _code(_HALF, x, "4-bit product operands")
-    if group not in (32, 64, 128) or x.dim() != 2 or x.shape[1] % group:
-        raise ValueError("weight group must be 32, 64 or 128 and divide the inner width")
-    inner = x.shape[1]
-    if codes.dim() != 3:
-        raise ValueError("4-bit weight codes must be [experts, outer, inner / 2]")
-    outer = codes.shape[1]
-    code_pointer = _packed(codes, (experts, outer, inner // 2), torch.uint8, "4-bit weight codes")
-    scale_pointer = _packed(scales, (experts, outer, inner // group), x.dtype, "4-bit weight scales")
-    entries = tokens * top_k
-    x_rows = tokens if gather else entries
-    address, stride = _rows(x, x_rows, inner, "x", gather)
-    out, result = _output(x, out, (entries, outer))
-    _matvec4(device, code, entries, experts, top_k, inner, outer, group, int(gather), address, x_rows, stride,
-             code_pointer, scale_pointer, rows, offsets, result)
-    return out
+    return _routed.routed_matvec(x, codes, scales, group, routing, gather, out)
