@@ -308,7 +308,8 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
       score = a.softmax != 0 ? __fdividef(expf(logit - top), total) : __fdividef(1.0f, 1.0f + expf(-logit));
       if (nan) score = __uint_as_float(0x7fc00000u);
     }
-    if (a.renormalize != 0) score = __fdividef(score, ChosenSum(score, a.top_k) + 1e-20f);
+    // (A single choice has the weight 1 exactly.)
+    if (a.renormalize != 0) score = __fdiv_rn(score, ChosenSum(score, a.top_k) + 1e-20f);
     if (lane < a.top_k) {
       a.chosen[entry] = mine;
       a.weights[entry] = mine < 0 ? 0.0f : score * a.scale;
@@ -554,9 +555,11 @@ __global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs
       p = __fdividef(1.0f, 1.0f + __expf(-logit));
     }
     if (a.renormalize != 0) {
-      const float total = __fdividef(1.0f, ChosenSum(p, a.top_k) + 1e-20f);
-      const float mean = ChosenSum(g * (p * total), a.top_k);
-      g = found ? (g - mean) * total : 0.0f;
+      // The weight is rounded as in the forward pass: a single choice's is 1 and
+      // its gradient 0, exactly.
+      const float total = ChosenSum(p, a.top_k) + 1e-20f;
+      const float mean = ChosenSum(g * __fdiv_rn(p, total), a.top_k);
+      g = found ? __fdividef(g - mean, total) : 0.0f;
     }
     if constexpr (kSoftmax) {
       const float inner = __shfl_sync(kFull, ChosenSum(g * p, a.top_k), 0);

@@ -232,6 +232,19 @@ def test_route_gradient_against_differences():
 
 
 @gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_a_single_renormalised_choice_is_exact(tokens, score):
+    """One expert of weight 1: no logit moves it."""
+    logits = torch.randn(tokens, 20, generator=torch.Generator().manual_seed(1)).cuda()
+    logits[:, 3:] -= 40.0 if tokens == 1 else 0.0
+    r = routed.route(logits, 1, score=score)
+    assert (r.weights == 1).all()
+    grad = routed.route_backward(logits, r, torch.randn(tokens, 1).cuda(), score=score)
+    assert (grad == 0).all()
+
+
+@gpu
 def test_route_surfaces_numbers_that_are_not():
     logits = torch.randn(3, 16).cuda()
     logits[0, 5] = math.nan
