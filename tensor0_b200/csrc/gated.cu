@@ -37,18 +37,26 @@ __device__ __forceinline__ bool RowWeight(const GatedArgs& a, int64_t p, float* 
   return true;
 }
 
-// Eight neighbours as they lie in memory, fetched ahead of their use.
+// A warp works on 256 columns of a row, eight per lane: neighbours in one
+// 16-byte access (Vector) where the rows allow it, otherwise every 32nd column,
+// so that a 2-byte access is still one 64-byte run of the warp.
+template <bool Vector>
+__device__ __forceinline__ int Column(int lane, int i) { return Vector ? lane * 8 + i : lane + 32 * i; }
+
+// Eight values as they lie in memory, fetched ahead of their use.  `row`: the
+// 256 columns' first, `left`: columns of the row from there on.
 template <typename T, bool Vector>
 struct Raw8 {
   uint4 bits;
-  __device__ __forceinline__ void Fetch(const T* p, int count) {
+  __device__ __forceinline__ void Fetch(const T* row, int left, int lane) {
     bits = make_uint4(0u, 0u, 0u, 0u);
     if constexpr (Vector) {
-      if (count > 0) bits = __ldcs(reinterpret_cast<const uint4*>(p));
+      if (lane * 8 < left) bits = __ldcs(reinterpret_cast<const uint4*>(row + lane * 8));
     } else {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
       uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = i < count ? reinterpret_cast<const uint16_t*>(p)[i] : 0u;
+      for (int i = 0; i < 8; ++i) w[i] = Column<false>(lane, i) < left ? p[Column<false>(lane, i)] : 0u;
       bits = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     }
   }
@@ -63,21 +71,38 @@ struct Raw8 {
   }
 };
 
+template <typename T, bool Vector>
+__device__ __forceinline__ void StoreRow(T* row, int left, int lane, const float (&v)[8]) {
+  if constexpr (Vector) {
+    Store8<T, true>(row + lane * 8, left - lane * 8, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (Column<false>(lane, i) < left) row[Column<false>(lane, i)] = FromFloat<T>(v[i]);
+    }
+  }
+}
+
 template <bool Vector>
 struct RawCodes {
   uint2 bits;
-  float unit;
-  __device__ __forceinline__ void Fetch(const int8_t* codes, const float* scale, int count) {
+  float unit[Vector ? 1 : 8];
+  // `scales`: of the 256 columns' first group.
+  __device__ __forceinline__ void Fetch(const int8_t* row, const float* scales, int shift, int left, int lane) {
     bits = make_uint2(0u, 0u);
-    unit = 0.0f;
-    if (count <= 0) return;
-    unit = *scale;
     if constexpr (Vector) {
-      bits = __ldcs(reinterpret_cast<const uint2*>(codes));
+      unit[0] = 0.0f;
+      if (lane * 8 >= left) return;
+      unit[0] = scales[(lane * 8) >> shift];
+      bits = __ldcs(reinterpret_cast<const uint2*>(row + lane * 8));
     } else {
       uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = i < count ? static_cast<uint8_t>(codes[i]) : 0u;
+      for (int i = 0; i < 8; ++i) {
+        const bool inside = Column<false>(lane, i) < left;
+        w[i] = inside ? static_cast<uint8_t>(row[Column<false>(lane, i)]) : 0u;
+        unit[i] = inside ? scales[(32 * i) >> shift] : 0.0f;
+      }
       bits = make_uint2(w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24);
     }
   }
@@ -87,40 +112,70 @@ struct RawCodes {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t word = __byte_perm(biased[i >> 2], 0x4b000000u, 0x7650 | (i & 3));
-      v[i] = (__uint_as_float(word) - 8388736.0f) * unit;
+      v[i] = (__uint_as_float(word) - 8388736.0f) * unit[Vector ? 0 : i];
     }
   }
 };
 
-// Codes of eight values and, by the group's first lane, the group's scale.
-// A NaN's magnitude bits are above infinity's, so the integer maximum keeps it.
+// A group's units per value and its scale, from the largest magnitude's bits.
+struct GroupScale {
+  float per_unit, scale;
+  __device__ __forceinline__ explicit GroupScale(uint32_t bits) {
+    const float largest = __uint_as_float(bits);
+    const bool none = largest < kSmallest;
+    per_unit = none ? 0.0f : __frcp_rn(largest) * 127.0f;
+    scale = none ? 0.0f : largest * (1.0f / 127.0f);
+  }
+};
+
+// |v * per_unit| is at most 127 and two roundings, so adding 1.5 * 2^23 rounds
+// it to a whole number, half to even, in the low byte (a group that is not
+// finite loads as NaN whatever its codes are).
+__device__ __forceinline__ uint32_t Code(float v, float per_unit) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(v, per_unit), 12582912.0f));
+}
+
+// Codes of the warp's 256 columns and the scales of their groups.  A NaN's
+// magnitude bits are above infinity's, so the integer maximum keeps it.
 template <bool Vector>
-__device__ __forceinline__ void StoreCodes(const float (&v)[8], int count, int lanes, int lane, int8_t* codes,
-                                           float* scale) {
-  uint32_t bits = 0;
+__device__ __forceinline__ void StoreCodes(const float (&v)[8], int left, int shift, int lane, int8_t* codes,
+                                           float* scales) {
+  uint32_t bits[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) bits = max(bits, __float_as_uint(v[i]) & 0x7fffffffu);
-  for (int d = lanes >> 1; d > 0; d >>= 1) bits = max(bits, __shfl_xor_sync(kFull, bits, d));
-  const float largest = __uint_as_float(bits);
-  const bool none = largest < kSmallest;
-  const float per_unit = none ? 0.0f : __frcp_rn(largest) * 127.0f;
-  if (count <= 0) return;
-  if ((lane & (lanes - 1)) == 0) *scale = none ? 0.0f : largest * (1.0f / 127.0f);
-  // |v * per_unit| is at most 127 and two roundings, so adding 1.5 * 2^23 rounds
-  // it to a whole number, half to even, in the low byte (a group that is not
-  // finite loads as NaN whatever its codes are).
-  uint32_t q[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], per_unit), 12582912.0f));
+  for (int i = 0; i < 8; ++i) bits[i] = __float_as_uint(v[i]) & 0x7fffffffu;
   if constexpr (Vector) {
+    const int lanes = 1 << (shift - 3);   // of a group
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, bits[i]);
+    for (int d = lanes >> 1; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(kFull, most, d));
+    const GroupScale group(most);
+    if (lane * 8 >= left) return;
+    if ((lane & (lanes - 1)) == 0) scales[(lane * 8) >> shift] = group.scale;
+    uint32_t q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = Code(v[i], group.per_unit);
     uint2 packed;
     packed.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
     packed.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
-    __stcs(reinterpret_cast<uint2*>(codes), packed);
+    __stcs(reinterpret_cast<uint2*>(codes + lane * 8), packed);
   } else {
+    // 32 neighbours per i; a group is 1, 2 or 4 of these.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits[i] = __reduce_max_sync(kFull, bits[i]);
+    if (shift >= 6) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) bits[i] = bits[i + 1] = max(bits[i], bits[i + 1]);
+    }
+    if (shift >= 7) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) bits[i] = bits[i + 1] = bits[i + 2] = bits[i + 3] = max(bits[i], bits[i + 2]);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i < count) codes[i] = static_cast<int8_t>(q[i] & 255u);
+      const GroupScale group(bits[i]);
+      if (lane == 0 && 32 * i < left && ((32 * i) & ((1 << shift) - 1)) == 0) scales[(32 * i) >> shift] = group.scale;
+      if (Column<false>(lane, i) < left) codes[Column<false>(lane, i)] = static_cast<int8_t>(Code(v[i], group.per_unit) & 255u);
     }
   }
 }
@@ -129,7 +184,7 @@ __device__ __forceinline__ void StoreCodes(const float (&v)[8], int count, int l
 // blockIdx.y is the part: few rows are split over their columns.
 template <typename T, bool Vector>
 __global__ void __launch_bounds__(kGatedThreads) GatedSave(GatedArgs a) {
-  const int lane = threadIdx.x & 31, lanes = a.group / 8, shift = 31 - __clz(a.group);
+  const int lane = threadIdx.x & 31, shift = 31 - __clz(a.group);
   const int groups = (a.width + a.group - 1) >> shift, stride = static_cast<int>(gridDim.y) * 256;
   const int64_t step = int64_t{gridDim.x} * (kGatedThreads / 32);
   for (int64_t p = int64_t{blockIdx.x} * (kGatedThreads / 32) + (threadIdx.x >> 5); p < a.rows_count; p += step) {
@@ -143,13 +198,13 @@ __global__ void __launch_bounds__(kGatedThreads) GatedSave(GatedArgs a) {
     const int begin = static_cast<int>(blockIdx.y) * 256;
     Raw8<T, Vector> next_g, next_u;
     const auto fetch = [&](int base) {
-      const int column = base + lane * 8, count = present ? a.width - column : 0;
-      next_g.Fetch(row + column, count);
-      next_u.Fetch(row + a.width + column, count);
+      const int left = present ? a.width - base : 0;
+      next_g.Fetch(row + base, left, lane);
+      next_u.Fetch(row + a.width + base, left, lane);
     };
     fetch(begin);
     for (int base = begin; base < a.width; base += stride) {
-      const int column = base + lane * 8, count = a.width - column;
+      const int left = a.width - base;
       float g[8], u[8], out[8];
       next_g.Values(g);
       next_u.Values(u);
@@ -160,10 +215,10 @@ __global__ void __launch_bounds__(kGatedThreads) GatedSave(GatedArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) out[i] = 0.0f;
       }
-      Store8<T, Vector>(out_row + column, count, out);
+      StoreRow<T, Vector>(out_row + base, left, lane, out);
       if (a.codes == nullptr) continue;   // the activation alone
-      StoreCodes<Vector>(g, count, lanes, lane, code_row + column, scale_row + (column >> shift));
-      StoreCodes<Vector>(u, count, lanes, lane, code_row + a.width + column, scale_row + groups + (column >> shift));
+      StoreCodes<Vector>(g, left, shift, lane, code_row + base, scale_row + (base >> shift));
+      StoreCodes<Vector>(u, left, shift, lane, code_row + a.width + base, scale_row + groups + (base >> shift));
     }
   }
 }
@@ -186,15 +241,15 @@ __global__ void __launch_bounds__(kGatedThreads) GatedBackward(GatedArgs a) {
     RawCodes<Vector> next_g, next_u;
     Raw8<T, Vector> next_da;
     const auto fetch = [&](int base) {
-      const int column = base + lane * 8, count = present ? a.width - column : 0;
-      next_g.Fetch(code_row + column, scale_row + (column >> shift), count);
-      next_u.Fetch(code_row + a.width + column, scale_row + groups + (column >> shift), count);
-      next_da.Fetch(grad_row + column, count);
+      const int left = present ? a.width - base : 0;
+      next_g.Fetch(code_row + base, scale_row + (base >> shift), shift, left, lane);
+      next_u.Fetch(code_row + a.width + base, scale_row + groups + (base >> shift), shift, left, lane);
+      next_da.Fetch(grad_row + base, left, lane);
     };
     fetch(0);
     float dot = 0.0f;
     for (int base = 0; base < a.width; base += 256) {
-      const int column = base + lane * 8, count = a.width - column;
+      const int left = a.width - base;
       float g[8], u[8], da[8], dg[8], du[8], out[8];
       next_g.Values(g);
       next_u.Values(u);
@@ -209,9 +264,9 @@ __global__ void __launch_bounds__(kGatedThreads) GatedBackward(GatedArgs a) {
         out[i] = weight * silu_u;
         dot = fmaf(da[i], silu_u, dot);
       }
-      Store8<T, Vector>(h_row + column, count, dg);
-      Store8<T, Vector>(h_row + a.width + column, count, du);
-      Store8<T, Vector>(out_row + column, count, out);
+      StoreRow<T, Vector>(h_row + base, left, lane, dg);
+      StoreRow<T, Vector>(h_row + a.width + base, left, lane, du);
+      StoreRow<T, Vector>(out_row + base, left, lane, out);
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
@@ -231,16 +286,23 @@ __global__ void __launch_bounds__(kGatedThreads) CheckpointLoad(GatedArgs a, T* 
     const int begin = static_cast<int>(blockIdx.y) * 256;
     RawCodes<Vector> next;
     const auto fetch = [&](int base) {
-      const int column = base + lane * 8;
-      next.Fetch(code_row + column, scale_row + (column >> shift), a.width - column);
+      next.Fetch(code_row + base, scale_row + (base >> shift), shift, a.width - base, lane);
     };
     fetch(begin);
     for (int base = begin; base < a.width; base += stride) {
-      const int column = base + lane * 8;
       float v[8];
       next.Values(v);
       if (base + stride < a.width) fetch(base + stride);
-      Store8<T, Vector && sizeof(T) == 2>(values + half * a.width + column, a.width - column, v);
+      T* row = values + half * a.width + base;
+      const int left = a.width - base;
+      if constexpr (Vector && sizeof(T) == 4) {
+        if (lane * 8 < left) {
+          reinterpret_cast<float4*>(row + lane * 8)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(row + lane * 8)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+      } else {
+        StoreRow<T, Vector>(row, left, lane, v);
+      }
     }
   }
 }
