@@ -102,6 +102,7 @@ uint64_t RequireRowWeights(const float* weights, const int32_t* row_entries, con
   Require(experts >= 1 && experts <= t0b::kRouteMaxExperts, "routed operators take 1 to 512 experts");
   Packed(weights, rows, 1, 4, "weight");
   Packed(row_entries, rows, 1, 4, "row");
+  if (rows != 0) Packed(offsets, experts + 1, 1, 4, "offset");
   return static_cast<uint64_t>(rows) * 4;
 }
 

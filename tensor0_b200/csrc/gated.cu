@@ -11,6 +11,7 @@
 // w is the row's routing weight (1 without a routing); rows that belong to no
 // expert are not read, and zeros are written for them.
 #include <algorithm>
+#include <type_traits>
 
 #include "engine.h"
 #include "layout.h"
@@ -24,7 +25,15 @@ constexpr uint32_t kFull = 0xffffffffu;
 constexpr int kGatedThreads = 256;
 constexpr float kSmallest = 0x1p-100f;   // 127 / m and m / 127 stay normal numbers above it
 
-__device__ __forceinline__ float Sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
+// 1 / (1 + exp(-g)) in four instructions, off by a few units in the last place
+// of 1 + exp(-g).  (Without .ftz each of the two special functions takes a
+// comparison and a scaling more; what they flush is far below the result's type.)
+__device__ __forceinline__ float Sigmoid(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
 
 // Row p's routing weight; false if the row belongs to no expert.
 __device__ __forceinline__ bool RowWeight(const GatedArgs& a, int64_t p, float* weight, int64_t* entry) {
@@ -47,26 +56,28 @@ __device__ __forceinline__ int Column(int lane, int i) { return Vector ? lane * 
 // 256 columns' first, `left`: columns of the row from there on.
 template <typename T, bool Vector>
 struct Raw8 {
-  uint4 bits;
+  uint32_t w[Vector ? 4 : 8];   // two values each, or one
   __device__ __forceinline__ void Fetch(const T* row, int left, int lane) {
-    bits = make_uint4(0u, 0u, 0u, 0u);
     if constexpr (Vector) {
-      if (lane * 8 < left) bits = __ldcs(reinterpret_cast<const uint4*>(row + lane * 8));
+      uint4 q = make_uint4(0u, 0u, 0u, 0u);
+      if (lane * 8 < left) q = __ldcs(reinterpret_cast<const uint4*>(row + lane * 8));
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
     } else {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-      uint32_t w[8];
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(row) + lane;
+      if (left >= 256) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = Column<false>(lane, i) < left ? p[Column<false>(lane, i)] : 0u;
-      bits = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        for (int i = 0; i < 8; ++i) w[i] = __ldcs(p + 32 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = lane + 32 * i < left ? __ldcs(p + 32 * i) : 0u;
+      }
     }
   }
   __device__ __forceinline__ void Values(float (&v)[8]) const {
-    const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Unpack2<T>(w[i]);
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (Vector) v[i] = (i & 1) == 0 ? Unpack2<T>(w[i / 2]).x : Unpack2<T>(w[i / 2]).y;
+      else v[i] = Unpack2<T>(w[i]).x;
     }
   }
 };
@@ -76,43 +87,51 @@ __device__ __forceinline__ void StoreRow(T* row, int left, int lane, const float
   if constexpr (Vector) {
     Store8<T, true>(row + lane * 8, left - lane * 8, v);
   } else {
+    T* p = row + lane;
+    if (left >= 256) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (Column<false>(lane, i) < left) row[Column<false>(lane, i)] = FromFloat<T>(v[i]);
+      for (int i = 0; i < 8; ++i) p[32 * i] = FromFloat<T>(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (lane + 32 * i < left) p[32 * i] = FromFloat<T>(v[i]);
+      }
     }
   }
 }
 
 template <bool Vector>
 struct RawCodes {
-  uint2 bits;
+  uint32_t w[Vector ? 2 : 8];   // four codes each, or one
   float unit[Vector ? 1 : 8];
   // `scales`: of the 256 columns' first group.
   __device__ __forceinline__ void Fetch(const int8_t* row, const float* scales, int shift, int left, int lane) {
-    bits = make_uint2(0u, 0u);
     if constexpr (Vector) {
       unit[0] = 0.0f;
+      w[0] = w[1] = 0u;
       if (lane * 8 >= left) return;
       unit[0] = scales[(lane * 8) >> shift];
-      bits = __ldcs(reinterpret_cast<const uint2*>(row + lane * 8));
+      const uint2 q = __ldcs(reinterpret_cast<const uint2*>(row + lane * 8));
+      w[0] = q.x;
+      w[1] = q.y;
     } else {
-      uint32_t w[8];
+      const uint8_t* p = reinterpret_cast<const uint8_t*>(row) + lane;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool inside = Column<false>(lane, i) < left;
-        w[i] = inside ? static_cast<uint8_t>(row[Column<false>(lane, i)]) : 0u;
-        unit[i] = inside ? scales[(32 * i) >> shift] : 0.0f;
+      for (int i = 0; i < 8; ++i) w[i] = lane + 32 * i < left ? __ldcs(p + 32 * i) : 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {   // one per group
+        const bool next = i == 0 || ((32 * i) & ((1 << shift) - 1)) == 0;
+        unit[i] = i != 0 && !next ? unit[i != 0 ? i - 1 : 0] : 32 * i < left ? scales[(32 * i) >> shift] : 0.0f;
       }
-      bits = make_uint2(w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24);
     }
   }
   // A byte c + 128 in the low bits of 2^23 is 2^23 + 128 + c: exact, without a conversion.
   __device__ __forceinline__ void Values(float (&v)[8]) const {
-    const uint32_t biased[2] = {bits.x ^ 0x80808080u, bits.y ^ 0x80808080u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t word = __byte_perm(biased[i >> 2], 0x4b000000u, 0x7650 | (i & 3));
-      v[i] = (__uint_as_float(word) - 8388736.0f) * unit[Vector ? 0 : i];
+      const uint32_t biased = w[Vector ? i >> 2 : i] ^ (Vector ? 0x80808080u : 0x80u);
+      const uint32_t word = __byte_perm(biased, 0x4b000000u, 0x7650 | (Vector ? i & 3 : 0));
+      v[i] = (__uint_as_float(Vector ? word : (biased | 0x4b000000u)) - 8388736.0f) * unit[Vector ? 0 : i];
     }
   }
 };
@@ -135,23 +154,27 @@ __device__ __forceinline__ uint32_t Code(float v, float per_unit) {
   return __float_as_uint(__fadd_rn(__fmul_rn(v, per_unit), 12582912.0f));
 }
 
-// Codes of the warp's 256 columns and the scales of their groups.  A NaN's
-// magnitude bits are above infinity's, so the integer maximum keeps it.
-template <bool Vector>
-__device__ __forceinline__ void StoreCodes(const float (&v)[8], int left, int shift, int lane, int8_t* codes,
-                                           float* scales) {
-  uint32_t bits[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bits[i] = __float_as_uint(v[i]) & 0x7fffffffu;
+// Two 16-bit values' larger magnitudes, NaN before everything.
+template <typename T>
+__device__ __forceinline__ uint32_t Larger2(uint32_t a, uint32_t b) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  const T2 r = __hmax2_nan(__habs2(*reinterpret_cast<const T2*>(&a)), __habs2(*reinterpret_cast<const T2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Codes of the warp's 256 columns and the scales of their groups of 1 << kShift.
+template <typename T, bool Vector, int kShift>
+__device__ __forceinline__ void StoreCodes(const Raw8<T, Vector>& raw, const float (&v)[8], int left, int lane,
+                                           int8_t* codes, float* scales) {
   if constexpr (Vector) {
-    const int lanes = 1 << (shift - 3);   // of a group
-    uint32_t most = 0;
+    constexpr int kLanes = 1 << (kShift - 3);   // of a group
+    uint32_t most = Larger2<T>(Larger2<T>(raw.w[0], raw.w[1]), Larger2<T>(raw.w[2], raw.w[3]));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, bits[i]);
-    for (int d = lanes >> 1; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(kFull, most, d));
-    const GroupScale group(most);
+    for (int d = kLanes >> 1; d > 0; d >>= 1) most = Larger2<T>(most, __shfl_xor_sync(kFull, most, d));
+    const float2 halves = Unpack2<T>(Larger2<T>(most, most >> 16));
+    const GroupScale group(__float_as_uint(halves.x) & 0x7fffffffu);
     if (lane * 8 >= left) return;
-    if ((lane & (lanes - 1)) == 0) scales[(lane * 8) >> shift] = group.scale;
+    if ((lane & (kLanes - 1)) == 0) scales[lane / kLanes] = group.scale;
     uint32_t q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = Code(v[i], group.per_unit);
@@ -160,72 +183,78 @@ __device__ __forceinline__ void StoreCodes(const float (&v)[8], int left, int sh
     packed.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
     __stcs(reinterpret_cast<uint2*>(codes + lane * 8), packed);
   } else {
-    // 32 neighbours per i; a group is 1, 2 or 4 of these.
+    // 32 neighbours per i; a group is 1, 2 or 4 of these.  Magnitudes compare as
+    // their bits do, where a NaN's are above infinity's.
+    constexpr int kRuns = 1 << (kShift - 5);
+    int8_t* p = codes + lane;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bits[i] = __reduce_max_sync(kFull, bits[i]);
-    if (shift >= 6) {
+    for (int i = 0; i < 8; i += kRuns) {
+      uint32_t most = 0;
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) bits[i] = bits[i + 1] = max(bits[i], bits[i + 1]);
-    }
-    if (shift >= 7) {
+      for (int j = 0; j < kRuns; ++j) most = max(most, raw.w[i + j] & 0x7fffu);
+      const GroupScale group(__float_as_uint(Unpack2<T>(__reduce_max_sync(kFull, most)).x));
+      if (lane == 0 && 32 * i < left) scales[i / kRuns] = group.scale;
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) bits[i] = bits[i + 1] = bits[i + 2] = bits[i + 3] = max(bits[i], bits[i + 2]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const GroupScale group(bits[i]);
-      if (lane == 0 && 32 * i < left && ((32 * i) & ((1 << shift) - 1)) == 0) scales[(32 * i) >> shift] = group.scale;
-      if (Column<false>(lane, i) < left) codes[Column<false>(lane, i)] = static_cast<int8_t>(Code(v[i], group.per_unit) & 255u);
+      for (int j = 0; j < kRuns; ++j) {
+        const int8_t code = static_cast<int8_t>(Code(v[i + j], group.per_unit) & 255u);
+        if (lane + 32 * (i + j) < left) p[32 * (i + j)] = code;
+      }
     }
   }
 }
 
-// The columns of a row that a warp takes: 256 at a time, every `parts`-th.
-// blockIdx.y is the part: few rows are split over their columns.
-template <typename T, bool Vector>
-__global__ void __launch_bounds__(kGatedThreads) GatedSave(GatedArgs a) {
-  const int lane = threadIdx.x & 31, shift = 31 - __clz(a.group);
-  const int groups = (a.width + a.group - 1) >> shift, stride = static_cast<int>(gridDim.y) * 256;
+// A warp takes 256 columns of a row at a time, every `parts`-th; blockIdx.y is
+// the part: few rows are split over their columns.  Bound by its instructions
+// as much as by memory (46 of them for a gate and an up value before the group
+// was a constant here and the rows' addresses were carried along).
+// Value by value there are too many registers for fetching ahead and for enough
+// warps; the warps are worth more.
+template <typename T, bool Vector, int kShift>
+__global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 4) GatedSave(GatedArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int groups = (a.width + (1 << kShift) - 1) >> kShift;
+  const int stride = static_cast<int>(gridDim.y) * 256, begin = static_cast<int>(blockIdx.y) * 256;
   const int64_t step = int64_t{gridDim.x} * (kGatedThreads / 32);
   for (int64_t p = int64_t{blockIdx.x} * (kGatedThreads / 32) + (threadIdx.x >> 5); p < a.rows_count; p += step) {
     float weight;
     int64_t entry;
     const bool present = RowWeight(a, p, &weight, &entry);
-    const T* row = static_cast<const T*>(a.h) + p * a.h_stride;
-    T* out_row = static_cast<T*>(a.a) + p * a.width;
-    int8_t* code_row = a.codes + p * 2 * a.width;
-    float* scale_row = a.scales + p * 2 * groups;
-    const int begin = static_cast<int>(blockIdx.y) * 256;
+    const T* h = static_cast<const T*>(a.h) + p * a.h_stride + begin;
+    T* out_row = static_cast<T*>(a.a) + p * a.width + begin;
+    int8_t* codes = a.codes + p * 2 * a.width + begin;
+    float* scales = a.scales + p * 2 * groups + (begin >> kShift);
     Raw8<T, Vector> next_g, next_u;
-    const auto fetch = [&](int base) {
-      const int left = present ? a.width - base : 0;
-      next_g.Fetch(row + base, left, lane);
-      next_u.Fetch(row + a.width + base, left, lane);
+    const auto fetch = [&](int left) {
+      next_g.Fetch(h, present ? left : 0, lane);
+      next_u.Fetch(h + a.width, present ? left : 0, lane);
+      h += stride;
     };
-    fetch(begin);
-    for (int base = begin; base < a.width; base += stride) {
-      const int left = a.width - base;
+    if (Vector) fetch(a.width - begin);
+    for (int left = a.width - begin; left > 0; left -= stride) {
+      if (!Vector) fetch(left);
+      const Raw8<T, Vector> raw_g = next_g, raw_u = next_u;
+      if (Vector && left > stride) fetch(left - stride);
       float g[8], u[8], out[8];
-      next_g.Values(g);
-      next_u.Values(u);
-      if (base + stride < a.width) fetch(base + stride);
+      raw_g.Values(g);
+      raw_u.Values(u);
+      // A row that is not present is zeros, whose activation is zero.
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = weight * (g[i] * Sigmoid(g[i])) * u[i];
-      if (!present) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = 0.0f;
+      for (int i = 0; i < 8; ++i) out[i] = (weight * g[i]) * Sigmoid(g[i]) * u[i];
+      StoreRow<T, Vector>(out_row, left, lane, out);
+      if (a.codes != nullptr) {   // null: the activation alone
+        StoreCodes<T, Vector, kShift>(raw_g, g, left, lane, codes, scales);
+        StoreCodes<T, Vector, kShift>(raw_u, u, left, lane, codes + a.width, scales + groups);
       }
-      StoreRow<T, Vector>(out_row + base, left, lane, out);
-      if (a.codes == nullptr) continue;   // the activation alone
-      StoreCodes<Vector>(g, left, shift, lane, code_row + base, scale_row + (base >> shift));
-      StoreCodes<Vector>(u, left, shift, lane, code_row + a.width + base, scale_row + groups + (base >> shift));
+      out_row += stride;
+      codes += stride;
+      scales += stride >> kShift;
     }
   }
 }
 
 // A warp takes a row: the routing weight's gradient is the row's sum.
 template <typename T, bool Vector>
-__global__ void __launch_bounds__(kGatedThreads) GatedBackward(GatedArgs a) {
+__global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 3) GatedBackward(GatedArgs a) {
   const int lane = threadIdx.x & 31, shift = 31 - __clz(a.group);
   const int groups = (a.width + a.group - 1) >> shift;
   const int64_t step = int64_t{gridDim.x} * (kGatedThreads / 32);
@@ -246,15 +275,16 @@ __global__ void __launch_bounds__(kGatedThreads) GatedBackward(GatedArgs a) {
       next_u.Fetch(code_row + a.width + base, scale_row + groups + (base >> shift), shift, left, lane);
       next_da.Fetch(grad_row + base, left, lane);
     };
-    fetch(0);
+    if (Vector) fetch(0);
     float dot = 0.0f;
     for (int base = 0; base < a.width; base += 256) {
+      if (!Vector) fetch(base);
       const int left = a.width - base;
       float g[8], u[8], da[8], dg[8], du[8], out[8];
       next_g.Values(g);
       next_u.Values(u);
       next_da.Values(da);
-      if (base + 256 < a.width) fetch(base + 256);
+      if (Vector && base + 256 < a.width) fetch(base + 256);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float s = Sigmoid(g[i]), silu = g[i] * s;
@@ -288,11 +318,12 @@ __global__ void __launch_bounds__(kGatedThreads) CheckpointLoad(GatedArgs a, T* 
     const auto fetch = [&](int base) {
       next.Fetch(code_row + base, scale_row + (base >> shift), shift, a.width - base, lane);
     };
-    fetch(begin);
+    if (Vector) fetch(begin);
     for (int base = begin; base < a.width; base += stride) {
+      if (!Vector) fetch(base);
       float v[8];
       next.Values(v);
-      if (base + stride < a.width) fetch(base + stride);
+      if (Vector && base + stride < a.width) fetch(base + stride);
       T* row = values + half * a.width + base;
       const int left = a.width - base;
       if constexpr (Vector && sizeof(T) == 4) {
@@ -318,12 +349,19 @@ dim3 RowBlocks(int64_t rows, int width) {
   return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(parts, 65535)));
 }
 
-template <typename T>
-void Save(const GatedArgs& a, cudaStream_t stream) {
+template <typename T, int kShift>
+void SaveGroups(const GatedArgs& a, cudaStream_t stream) {
   const bool vector = a.width % 8 == 0 && a.h_stride % 8 == 0 && Aligned(a.h, 16) && Aligned(a.a, 16) && Aligned(a.codes, 8);
   const dim3 blocks = RowBlocks(a.rows_count, a.width);
-  if (vector) GatedSave<T, true><<<blocks, kGatedThreads, 0, stream>>>(a);
-  else GatedSave<T, false><<<blocks, kGatedThreads, 0, stream>>>(a);
+  if (vector) GatedSave<T, true, kShift><<<blocks, kGatedThreads, 0, stream>>>(a);
+  else GatedSave<T, false, kShift><<<blocks, kGatedThreads, 0, stream>>>(a);
+}
+
+template <typename T>
+void Save(const GatedArgs& a, cudaStream_t stream) {
+  if (a.group == 128) SaveGroups<T, 7>(a, stream);
+  else if (a.group == 64) SaveGroups<T, 6>(a, stream);
+  else SaveGroups<T, 5>(a, stream);
 }
 
 template <typename T>
