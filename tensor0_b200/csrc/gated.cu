@@ -23,6 +23,7 @@ namespace {
 
 constexpr uint32_t kFull = 0xffffffffu;
 constexpr int kGatedThreads = 256;
+constexpr const char* kLaunch = "gated activation launch";
 constexpr float kSmallest = 0x1p-100f;   // 127 / m and m / 127 stay normal numbers above it
 
 // 1 / (1 + exp(-g)) in four instructions, off by a few units in the last place
@@ -211,6 +212,8 @@ __device__ __forceinline__ void StoreCodes(const Raw8<T, Vector>& raw, const flo
 // warps; the warps are worth more.
 template <typename T, bool Vector, int kShift>
 __global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 4) GatedSave(GatedArgs a) {
+  LetNextStart();
+  WaitForPrevious();
   const int lane = threadIdx.x & 31;
   const int groups = (a.width + (1 << kShift) - 1) >> kShift;
   const int stride = static_cast<int>(gridDim.y) * 256, begin = static_cast<int>(blockIdx.y) * 256;
@@ -255,6 +258,8 @@ __global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 4) GatedSave(Gated
 // A warp takes a row: the routing weight's gradient is the row's sum.
 template <typename T, bool Vector>
 __global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 3) GatedBackward(GatedArgs a) {
+  LetNextStart();
+  WaitForPrevious();
   const int lane = threadIdx.x & 31, shift = 31 - __clz(a.group);
   const int groups = (a.width + a.group - 1) >> shift;
   const int64_t step = int64_t{gridDim.x} * (kGatedThreads / 32);
@@ -306,6 +311,8 @@ __global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 3) GatedBackward(G
 
 template <typename T, bool Vector>
 __global__ void __launch_bounds__(kGatedThreads) CheckpointLoad(GatedArgs a, T* values) {
+  LetNextStart();
+  WaitForPrevious();
   const int lane = threadIdx.x & 31, shift = 31 - __clz(a.group);
   const int groups = (a.width + a.group - 1) >> shift, stride = static_cast<int>(gridDim.y) * 256;
   const int64_t halves = a.rows_count * 2, step = int64_t{gridDim.x} * (kGatedThreads / 32);
@@ -353,8 +360,8 @@ template <typename T, int kShift>
 void SaveGroups(const GatedArgs& a, cudaStream_t stream) {
   const bool vector = a.width % 8 == 0 && a.h_stride % 8 == 0 && Aligned(a.h, 16) && Aligned(a.a, 16) && Aligned(a.codes, 8);
   const dim3 blocks = RowBlocks(a.rows_count, a.width);
-  if (vector) GatedSave<T, true, kShift><<<blocks, kGatedThreads, 0, stream>>>(a);
-  else GatedSave<T, false, kShift><<<blocks, kGatedThreads, 0, stream>>>(a);
+  if (vector) LaunchRouted(kLaunch, BriefGrid(int64_t{blocks.x} * blocks.y), GatedSave<T, true, kShift>, blocks, kGatedThreads, 0, stream, a);
+  else LaunchRouted(kLaunch, BriefGrid(int64_t{blocks.x} * blocks.y), GatedSave<T, false, kShift>, blocks, kGatedThreads, 0, stream, a);
 }
 
 template <typename T>
@@ -369,21 +376,17 @@ void Backward(const GatedArgs& a, cudaStream_t stream) {
   const bool vector = a.width % 8 == 0 && a.a_grad_stride % 8 == 0 && Aligned(a.a_grad, 16) && Aligned(a.a, 16) &&
                       Aligned(a.h_grad, 16) && Aligned(a.codes, 8);
   const unsigned blocks = RowBlocks(a.rows_count, 1).x;
-  if (vector) GatedBackward<T, true><<<blocks, kGatedThreads, 0, stream>>>(a);
-  else GatedBackward<T, false><<<blocks, kGatedThreads, 0, stream>>>(a);
+  if (vector) LaunchRouted(kLaunch, BriefGrid(blocks), GatedBackward<T, true>, blocks, kGatedThreads, 0, stream, a);
+  else LaunchRouted(kLaunch, BriefGrid(blocks), GatedBackward<T, false>, blocks, kGatedThreads, 0, stream, a);
 }
 
 template <typename T>
 void Load(const GatedArgs& a, void* values, cudaStream_t stream) {
   const bool vector = a.width % 8 == 0 && Aligned(values, 16) && Aligned(a.codes, 8);
   const dim3 blocks = RowBlocks(a.rows_count * 2, a.width);
-  if (vector) CheckpointLoad<T, true><<<blocks, kGatedThreads, 0, stream>>>(a, static_cast<T*>(values));
-  else CheckpointLoad<T, false><<<blocks, kGatedThreads, 0, stream>>>(a, static_cast<T*>(values));
-}
-
-void Launched() {
-  Check(cudaGetLastError(), "gated activation launch");
-  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  T* to = static_cast<T*>(values);
+  if (vector) LaunchRouted(kLaunch, BriefGrid(int64_t{blocks.x} * blocks.y), CheckpointLoad<T, true>, blocks, kGatedThreads, 0, stream, a, to);
+  else LaunchRouted(kLaunch, BriefGrid(int64_t{blocks.x} * blocks.y), CheckpointLoad<T, false>, blocks, kGatedThreads, 0, stream, a, to);
 }
 
 }  // namespace
@@ -392,14 +395,12 @@ void LaunchGatedSave(int32_t dtype, const GatedArgs& args, cudaStream_t stream) 
   if (dtype == kTypeF16) Save<__half>(args, stream);
   else if (dtype == kTypeBf16) Save<__nv_bfloat16>(args, stream);
   else throw InvalidArgument("gated activations take F16 or BF16");
-  Launched();
 }
 
 void LaunchGatedBackward(int32_t dtype, const GatedArgs& args, cudaStream_t stream) {
   if (dtype == kTypeF16) Backward<__half>(args, stream);
   else if (dtype == kTypeBf16) Backward<__nv_bfloat16>(args, stream);
   else throw InvalidArgument("gated activations take F16 or BF16");
-  Launched();
 }
 
 void LaunchCheckpointLoad(int32_t dtype, const GatedArgs& args, void* values, cudaStream_t stream) {
@@ -407,7 +408,6 @@ void LaunchCheckpointLoad(int32_t dtype, const GatedArgs& args, void* values, cu
   else if (dtype == kTypeBf16) Load<__nv_bfloat16>(args, values, stream);
   else if (dtype == kTypeF32) Load<float>(args, values, stream);
   else throw InvalidArgument("checkpoints load as F32, F16 or BF16");
-  Launched();
 }
 
 }  // namespace t0b

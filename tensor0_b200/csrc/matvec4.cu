@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
   const int x_size = max_rows * kMvStride, sum_size = (max_rows + 1) / 2 * 2 * kChunkGroups;
   float* x_sums = reinterpret_cast<float*>(x_values + 2 * x_size);
   uint16_t* scales = reinterpret_cast<uint16_t*>(x_sums + 2 * sum_size);
+  LetNextStart();
   if (tid == 0) {
     for (int i = 0; i < kMvStages; ++i) {
       BarrierInit(SharedAddress(&s.full[i]), 1);
@@ -159,6 +160,8 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
     s.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == 32) PrefetchMap(&map);
+  WaitForPrevious();
   if (warp == 0) {
     int seen = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
@@ -462,10 +465,8 @@ void Launch(const MatvecArgs& a, cudaStream_t stream) {
   const CUtensorMap map = EncodeBytes(a.codes, a.inner / 2, int64_t{a.experts} * a.outer, 128, kRows);
   AllowShared<Matvec<T, kGroup, kParts>>(smem);
   const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, RoutedSmCount() * 2));
-  Matvec<T, kGroup, kParts><<<grid, kMvThreads + 32 + kMvLayout, smem, stream>>>(a, map, row_blocks, rows, vector,
-                                                                               vector_scales);
-  Check(cudaGetLastError(), "4-bit product launch");
-  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  LaunchRouted("4-bit product launch", BriefGrid(blocks), Matvec<T, kGroup, kParts>, grid, kMvThreads + 32 + kMvLayout, smem, stream, a, map,
+               row_blocks, rows, vector, vector_scales);
 }
 
 template <typename T, int kGroup>

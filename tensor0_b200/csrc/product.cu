@@ -23,6 +23,8 @@ constexpr int kGenTile = 64, kGenDeep = 16, kGenThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kGenThreads) GeneralProduct(ProductArgs a, int kind) {
   __shared__ float left[kGenDeep][kGenTile + 4], right[kGenDeep][kGenTile + 4];
+  LetNextStart();
+  WaitForPrevious();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const T* x = static_cast<const T*>(a.x);
   const T* w = static_cast<const T*>(a.w);
@@ -109,6 +111,8 @@ __global__ void __launch_bounds__(kGenThreads) GeneralProduct(ProductArgs a, int
 // read once, four rows in flight.
 template <typename T, bool Vector>
 __global__ void __launch_bounds__(256) RoutedSum(RoutedSumArgs a) {
+  LetNextStart();
+  WaitForPrevious();
   const int column = static_cast<int>(blockIdx.y) * 256 + (threadIdx.x & 31) * 8, count = a.width - column;
   const T* y = static_cast<const T*>(a.y) + column;
   const int64_t step = int64_t{gridDim.x} * 8;
@@ -134,9 +138,8 @@ __global__ void __launch_bounds__(256) RoutedSum(RoutedSumArgs a) {
 
 template <typename T>
 void Launch(int kind, const ProductArgs& a, cudaStream_t stream) {
-  GeneralProduct<T><<<static_cast<unsigned>(RoutedSmCount() * 4), kGenThreads, 0, stream>>>(a, kind);
-  Check(cudaGetLastError(), "routed product launch");
-  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  LaunchRouted("routed product launch", false, GeneralProduct<T>, static_cast<unsigned>(RoutedSmCount() * 4), kGenThreads, 0,
+               stream, a, kind);
 }
 
 template <typename T>
@@ -146,10 +149,10 @@ void Sum(const RoutedSumArgs& a, cudaStream_t stream) {
                     static_cast<unsigned>((a.width + 255) / 256));   // a width is at most 2^23
   const bool vector = a.width % 8 == 0 && a.y_stride % 8 == 0 && a.out_stride % 8 == 0 &&
                       reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
-  if (vector) RoutedSum<T, true><<<blocks, 256, 0, stream>>>(a);
-  else RoutedSum<T, false><<<blocks, 256, 0, stream>>>(a);
-  Check(cudaGetLastError(), "routed sum launch");
-  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  const char* what = "routed sum launch";
+  const bool brief = BriefGrid(int64_t{blocks.x} * blocks.y);
+  if (vector) LaunchRouted(what, brief, RoutedSum<T, true>, blocks, 256, 0, stream, a);
+  else LaunchRouted(what, brief, RoutedSum<T, false>, blocks, 256, 0, stream, a);
 }
 
 }  // namespace

@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
   const int tiles_n = (width + kWide - 1) / kWide;
   constexpr uint32_t kTmemColumns = 2 * kWide;
 
+  LetNextStart();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SharedAddress(&s.tmem)),
                  "r"(kTmemColumns) : "memory");
@@ -138,6 +139,11 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
     s.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == 32) {
+    PrefetchMap(&a.a);
+    PrefetchMap(&a.b);
+  }
+  WaitForPrevious();
   for (int e = tid; e <= a.experts; e += blockDim.x) {
     s.row_begin[e] = static_cast<int>(RowBound(a.offsets[e], a.entries));
   }
@@ -486,9 +492,8 @@ void LaunchTc(const ProductArgs& p, bool bf16, int64_t tiles, int sms, cudaStrea
   constexpr int smem = static_cast<int>(Shape::kRing + 4 * kStagingBytes) + 1024;
   AllowShared<TcProduct<kKind, kWide, kGather>>(smem);
   const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(tiles, sms)));
-  TcProduct<kKind, kWide, kGather><<<grid, kTcThreads + (kGather ? kGatherThreads : 0), smem, stream>>>(a);
-  Check(cudaGetLastError(), "routed product launch");
-  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  LaunchRouted("routed product launch", tiles <= sms, TcProduct<kKind, kWide, kGather>, grid,
+               kTcThreads + (kGather ? kGatherThreads : 0), smem, stream, a);
 }
 
 template <int kKind>

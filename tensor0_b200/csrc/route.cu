@@ -396,6 +396,8 @@ __device__ __forceinline__ void CountEntries(const RouteArgs& a, int64_t begin, 
 template <typename T, int V, bool kByLogit>
 __global__ void __launch_bounds__(1024) RouteOneBlock(RouteArgs a, bool vector) {
   extern __shared__ int route_smem[];
+  LetNextStart();
+  WaitForPrevious();
   int* first = route_smem;                        // experts + 1
   int* by_warp = first + a.experts + 1;           // warps x (experts + 1)
   float* values = reinterpret_cast<float*>(by_warp);   // reused: the choice is over before rows are placed
@@ -410,15 +412,11 @@ __global__ void __launch_bounds__(1024) RouteOneBlock(RouteArgs a, bool vector) 
   PlaceEntries(a, 0, a.tokens * a.top_k, first, by_warp);
 }
 
-// The three launches overlap: each starts while the one before it ends, and
-// waits for its writes here.
-__device__ __forceinline__ void LetNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void WaitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 template <typename T, int V, bool kByLogit>
 __global__ void __launch_bounds__(kRouteThreads) RouteSelect(RouteArgs a, int64_t tokens_per_block, bool vector) {
   extern __shared__ int route_smem[];
   LetNextStart();
+  WaitForPrevious();
   int* bins = route_smem;
   float* values = reinterpret_cast<float*>(bins + a.experts);
   for (int e = threadIdx.x; e < a.experts; e += blockDim.x) bins[e] = 0;
@@ -480,6 +478,7 @@ __global__ void __launch_bounds__(kPlaceThreads) RoutePlace(RouteArgs a, int64_t
   extern __shared__ int route_smem[];
   int* first = route_smem;                  // experts + 1
   int* by_warp = first + a.experts + 1;
+  LetNextStart();
   WaitForPrevious();
   const int32_t* totals = a.counts + gridDim.x * int64_t{a.experts};
   for (int e = threadIdx.x; e < a.experts; e += kPlaceThreads) first[e] = totals[e];
@@ -520,6 +519,8 @@ __global__ void __launch_bounds__(kPlaceThreads) RoutePlace(RouteArgs a, int64_t
 template <typename T, int V, bool kSoftmax>
 __global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs a, bool vector) {
   __shared__ __align__(16) float scattered[kRouteThreads / 32][32 * V];   // ds
+  LetNextStart();
+  WaitForPrevious();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = static_cast<int>(blockIdx.x) * (kRouteThreads / 32) + warp;   // tokens * top_k is below 2^31
   if (t >= static_cast<int>(a.tokens)) return;
@@ -589,22 +590,6 @@ int64_t TokensPerBlock(int64_t tokens) {
   return std::max<int64_t>(8, ((tokens + blocks - 1) / blocks + 7) / 8 * 8);
 }
 
-template <typename... Args>
-void LaunchAfter(void (*kernel)(Args...), unsigned blocks, unsigned threads, std::size_t smem, cudaStream_t stream,
-                 Args... args) {
-  cudaLaunchAttribute overlap{};
-  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  overlap.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(blocks);
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = smem;
-  config.stream = stream;
-  config.attrs = &overlap;
-  config.numAttrs = 1;
-  Check(cudaLaunchKernelEx(&config, kernel, args...), "row order launch");
-}
-
 template <typename T, int V, bool kByLogit>
 void Route(const RouteArgs& a, cudaStream_t stream) {
   const std::size_t bins = static_cast<std::size_t>(a.experts) + 1;
@@ -613,30 +598,26 @@ void Route(const RouteArgs& a, cudaStream_t stream) {
     const unsigned warps = static_cast<unsigned>(std::min<int64_t>(32, std::max<int64_t>(1, a.tokens)));
     const std::size_t smem = (bins + warps * bins) * sizeof(int);
     AllowShared<RouteOneBlock<T, V, kByLogit>>(static_cast<int>(smem));
-    RouteOneBlock<T, V, kByLogit><<<1, warps * 32, smem, stream>>>(a, vector);
-    Check(cudaGetLastError(), "router launch");
-    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+    LaunchRouted("router launch", true, RouteOneBlock<T, V, kByLogit>, 1, warps * 32, smem, stream, a, vector);
     return;
   }
   const int64_t per_block = TokensPerBlock(a.tokens);
   const unsigned blocks = static_cast<unsigned>((a.tokens + per_block - 1) / per_block);
   const std::size_t select = (bins + (a.groups > 1 ? kRouteThreads / 32 * bins : 0)) * sizeof(int);
-  RouteSelect<T, V, kByLogit><<<blocks, kRouteThreads, select, stream>>>(a, per_block, vector);
-  Check(cudaGetLastError(), "router launch");
-  LaunchAfter(RouteScan, static_cast<unsigned>((a.experts + kScanExperts - 1) / kScanExperts), kScanThreads, 0, stream, a,
-              static_cast<int>(blocks));
-  LaunchAfter(RoutePlace, blocks, kPlaceThreads, (1 + kPlaceThreads / 32) * bins * sizeof(int), stream, a, per_block);
-  g_kernel_launches.fetch_add(3, std::memory_order_relaxed);
+  LaunchRouted("router launch", BriefGrid(blocks), RouteSelect<T, V, kByLogit>, blocks, kRouteThreads, select, stream, a, per_block, vector);
+  LaunchRouted("row order launch", BriefGrid(blocks), RouteScan, static_cast<unsigned>((a.experts + kScanExperts - 1) / kScanExperts),
+               kScanThreads, 0, stream, a, static_cast<int>(blocks));
+  LaunchRouted("row order launch", BriefGrid(blocks), RoutePlace, blocks, kPlaceThreads, (1 + kPlaceThreads / 32) * bins * sizeof(int),
+               stream, a, per_block);
 }
 
 template <typename T, int V>
 void Backward(const RouteBackwardArgs& a, cudaStream_t stream) {
   const unsigned blocks = static_cast<unsigned>((a.tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32));
   const bool vector = VectorLogits<T, V>(a.logits, a.logit_stride) && VectorLogits<T, V>(a.logits_grad, a.experts);
-  if (a.softmax != 0) RouteBackward<T, V, true><<<blocks, kRouteThreads, 0, stream>>>(a, vector);
-  else RouteBackward<T, V, false><<<blocks, kRouteThreads, 0, stream>>>(a, vector);
-  Check(cudaGetLastError(), "router gradient launch");
-  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  const char* what = "router gradient launch";
+  if (a.softmax != 0) LaunchRouted(what, BriefGrid(blocks), RouteBackward<T, V, true>, blocks, kRouteThreads, 0, stream, a, vector);
+  else LaunchRouted(what, BriefGrid(blocks), RouteBackward<T, V, false>, blocks, kRouteThreads, 0, stream, a, vector);
 }
 
 template <typename T, typename Args, typename Body>

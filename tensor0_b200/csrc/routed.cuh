@@ -5,7 +5,9 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <cstddef>
 #include <cstdint>
+#include <utility>
 
 #include "engine.h"
 
@@ -90,6 +92,37 @@ __device__ __forceinline__ int64_t RowBound(int32_t offset, int64_t entries) {
   return offset < 0 ? 0 : offset < entries ? offset : entries;
 }
 
+// Brief kernels follow one another closely: each lets the next one start (and
+// set itself up) while it runs, and waits for the one before it to have ended,
+// with its writes, before it touches memory.  Every block of every kernel waits,
+// so that a kernel's end implies the end of all before it.
+__device__ __forceinline__ void LetNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void WaitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches a kernel that begins with these two.  brief: it may start while the
+// kernel before it runs.  That takes 0.3 to 0.8 us off calls of 4 to 8 us (a
+// route of 8 tokens, a product of 64), and costs long ones a few percent (the
+// product and sum of 8192 tokens 172 us instead of 166), so those do without.
+template <typename... Parameters, typename... Arguments>
+void LaunchRouted(const char* what, bool brief, void (*kernel)(Parameters...), dim3 blocks, unsigned threads, std::size_t smem,
+                  cudaStream_t stream, Arguments&&... arguments) {
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = blocks;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &overlap;
+  config.numAttrs = brief ? 1 : 0;
+  Check(cudaLaunchKernelEx(&config, kernel, std::forward<Arguments>(arguments)...), what);
+  g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+}
+
+// Whether a kernel of that many blocks is over in about one turn.
+inline bool BriefGrid(int64_t blocks);
+
 // The current device, and its streaming multiprocessors (asked for once).
 constexpr int kMaxDevices = 64;
 
@@ -108,6 +141,8 @@ inline int RoutedSmCount() {
   }
   return count;
 }
+
+inline bool BriefGrid(int64_t blocks) { return blocks <= 2 * RoutedSmCount(); }
 
 // Lets kernel `kKernel` use `bytes` of dynamic shared memory on the current
 // device; asked for once per device and size, since the call costs as much as

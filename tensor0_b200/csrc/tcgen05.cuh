@@ -53,6 +53,11 @@ __device__ __forceinline__ bool BarrierWait(uint32_t bar, uint32_t parity, volat
   return true;
 }
 
+// Brings a tensor map (a kernel parameter) near before its first use.
+__device__ __forceinline__ void PrefetchMap(const void* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 __device__ __forceinline__ void LoadTile2(uint32_t dst, const void* map, uint32_t bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
