@@ -604,10 +604,13 @@ void Route(const RouteArgs& a, cudaStream_t stream) {
   const int64_t per_block = TokensPerBlock(a.tokens);
   const unsigned blocks = static_cast<unsigned>((a.tokens + per_block - 1) / per_block);
   const std::size_t select = (bins + (a.groups > 1 ? kRouteThreads / 32 * bins : 0)) * sizeof(int);
+  // While the choice is short, the two launches after it are worth hiding (8191
+  // tokens: 27 us instead of 31; 32768: 56 instead of 54).
+  const bool close = per_block <= 16;
   LaunchRouted("router launch", BriefGrid(blocks), RouteSelect<T, V, kByLogit>, blocks, kRouteThreads, select, stream, a, per_block, vector);
-  LaunchRouted("row order launch", BriefGrid(blocks), RouteScan, static_cast<unsigned>((a.experts + kScanExperts - 1) / kScanExperts),
+  LaunchRouted("row order launch", close, RouteScan, static_cast<unsigned>((a.experts + kScanExperts - 1) / kScanExperts),
                kScanThreads, 0, stream, a, static_cast<int>(blocks));
-  LaunchRouted("row order launch", BriefGrid(blocks), RoutePlace, blocks, kPlaceThreads, (1 + kPlaceThreads / 32) * bins * sizeof(int),
+  LaunchRouted("row order launch", close, RoutePlace, blocks, kPlaceThreads, (1 + kPlaceThreads / 32) * bins * sizeof(int),
                stream, a, per_block);
 }
 
