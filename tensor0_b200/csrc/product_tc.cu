@@ -19,6 +19,15 @@
 // shared memory and not stored (experts with few rows load few).  In the weight gradient they would enter the sum: the
 // matrix warp zeroes them in shared memory, in both operands, so that a value
 // that is not finite stays with its own expert.
+//
+// Measured, bf16: 32768 rows of 64 experts, 1024 x 2048, 138 us (1.0 PFLOP/s,
+// 0.62 of the matrix rate; every second expert's last tile is half empty); of 32
+// experts at 2048 x 2048 230 us (1.2); that weight gradient 255 us, with gathered
+// rows 330.  9222 rows of 40 experts at 1000 x 1416 f16 49 us, where reading the
+// weights takes 17.  What bounds: the slices' latency against four stages, and at
+// few rows per expert the weights' bytes.
+// Two blocks sharing 256 x 256 tiles (cta_group::2) were slower: 265 us where
+// this takes 232, for the tiles' empty halves and the blocks' handshakes.
 #include <algorithm>
 
 #include "engine.h"
