@@ -10,11 +10,9 @@
 // A logit of -inf or NaN, and a masked token, take no expert (index -1,
 // weight 0).  Under softmax a NaN or +inf logit makes the row's weights NaN.
 //
-// One warp holds a token: lane l has the kV experts from l * kV on.  A pick is a
-// warp reduction of the choice values as ordered integers and a ballot: the
-// first lane that holds the largest has the lowest index.  Bound by these
-// instructions, not by memory, so nothing else is done for all experts where it
-// can be done for the chosen ones: without a bias the scores are taken of those
+// One warp holds a token: lane l has the V experts from l * V on.  Bound by
+// instructions, not by memory, so nothing is done for all experts where it can
+// be done for the chosen ones: without a bias the scores are taken of those
 // alone, and where the weights are renormalised the softmax needs no sum over
 // all experts.
 //
@@ -23,7 +21,7 @@
 // one block that does it all.
 //
 // Measured: 8 tokens of 64 experts 3.8 us; 8191 of 256 in groups with a bias
-// 24 us (choice 17); 32768 of 128 forward and backward 44 us (choice 26,
+// 24 us (choice 17); 32768 of 128 forward and backward 41 us (choice 24,
 // gradient 11, where reading and writing the logits takes 6).
 #include <algorithm>
 #include <climits>
@@ -141,11 +139,6 @@ __device__ __forceinline__ float Largest(const float (&x)[V]) {
   return WarpMax(top);
 }
 
-// Inverse of Ordered.
-__device__ __forceinline__ float Unordered(uint32_t key) {
-  return __uint_as_float((key >> 31) != 0 ? key ^ 0x80000000u : ~key);
-}
-
 // Of each group of `size` experts the best value, or the sum of its two best;
 // lane g has group g's.  `values`: one row per warp of shared memory.
 template <int V>
@@ -184,6 +177,83 @@ __device__ __forceinline__ float GroupScore(const float (&c)[V], int experts, in
   }
   if (best == 2 && second > -INFINITY) first += second;
   return __shfl_sync(kFull, first, source & 31);
+}
+
+// Batcher's merge exchange sort of a lane's numbers, largest first.
+template <int V>
+__device__ __forceinline__ void SortDescending(uint32_t (&k)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2) {
+#pragma unroll
+    for (int d = p; d >= 1; d /= 2) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const bool first = d == p ? j % (2 * p) < p : j >= d && (j - d) % (2 * d) < d;
+        if (first && j + d < V && j / (2 * p) == (j + d) / (2 * p)) {
+          const uint32_t high = max(k[j], k[j + d]), low = min(k[j], k[j + d]);
+          k[j] = high;
+          k[j + d] = low;
+        }
+      }
+    }
+  }
+}
+
+// The expert of slot `lane` by all bits of the choice values (0: not eligible).
+// A pick is a warp reduction and a ballot: the first lane that holds the largest
+// has the lowest index.
+template <int V>
+__device__ __forceinline__ int PickExactly(uint32_t (&key)[V], int top_k) {
+  const int lane = threadIdx.x & 31;
+  int mine = -1;
+#pragma unroll 1
+  for (int n = 0; n < top_k; ++n) {
+    uint32_t best = key[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) best = max(best, key[j]);
+    const uint32_t largest = __reduce_max_sync(kFull, best);
+    if (largest == 0u) break;
+    const int winner = __ffs(__ballot_sync(kFull, best == largest)) - 1;
+    int at = V - 1;
+#pragma unroll
+    for (int j = V - 2; j >= 0; --j) at = key[j] == largest ? j : at;
+    const int index = __shfl_sync(kFull, lane * V + at, winner);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (lane * V + j == index) key[j] = 0u;
+    }
+    if (lane == n) mine = index;
+  }
+  return mine;
+}
+
+// The same by one number for each expert, the choice value's high bits and the
+// expert (lower ones first): every lane sorts its own, and a pick is one
+// reduction and the winner's next.  Values that the high bits do not tell apart
+// are next to each other in that order; *close: there is such a pair up to the
+// first value not taken, and the picks may not be the ones by all bits.
+template <int V>
+__device__ __forceinline__ int PickPacked(const uint32_t (&key)[V], int top_k, bool* close) {
+  constexpr uint32_t kIndex = 32 * V - 1;
+  const int lane = threadIdx.x & 31;
+  uint32_t packed[V], pick = 0u, previous = 0u;
+#pragma unroll
+  for (int j = 0; j < V; ++j) packed[j] = (key[j] & ~kIndex) | (kIndex - static_cast<uint32_t>(lane * V + j));
+  SortDescending<V>(packed);
+  *close = false;
+#pragma unroll 1
+  for (int n = 0; n <= top_k; ++n) {
+    const uint32_t largest = __reduce_max_sync(kFull, packed[0]);
+    if (largest <= kIndex) break;
+    *close = *close || (largest ^ previous) <= kIndex;
+    previous = largest;
+    if (lane == n) pick = largest;
+    const bool winner = packed[0] == largest;
+#pragma unroll
+    for (int j = 0; j + 1 < V; ++j) packed[j] = winner ? packed[j + 1] : packed[j];
+    packed[V - 1] = winner ? 0u : packed[V - 1];
+  }
+  return lane < top_k && pick != 0u ? static_cast<int>(kIndex - (pick & kIndex)) : -1;
 }
 
 // Chosen experts and weights of the block's tokens.  kByLogit: the choice goes
@@ -282,32 +352,18 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
       }
     }
     int mine = -1;
-    uint32_t mine_key = 0;
-#pragma unroll 1
-    for (int n = 0; n < a.top_k; ++n) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int j = 1; j < V; ++j) best = max(best, key[j]);
-      const uint32_t largest = __reduce_max_sync(kFull, best);
-      if (largest == 0u) break;
-      const int winner = __ffs(__ballot_sync(kFull, best == largest)) - 1;
-      int at = V - 1;
-#pragma unroll
-      for (int j = V - 2; j >= 0; --j) at = key[j] == largest ? j : at;
-      const int index = __shfl_sync(kFull, lane * V + at, winner);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (lane * V + j == index) key[j] = 0u;
-      }
-      if (lane == n) {
-        mine = index;
-        mine_key = largest;
-      }
+    if constexpr (kByLogit) {
+      bool close;
+      mine = PickPacked<V>(key, a.top_k, &close);
+      // 16-bit logits that are not equal differ in the bits that were compared.
+      if (sizeof(T) == 4 && close) mine = PickExactly<V>(key, a.top_k);
+    } else {
+      mine = PickExactly<V>(key, a.top_k);   // (packed: 25 us for 8191 tokens instead of 23.5)
     }
+    const float logit = mine >= 0 ? ToFloat(row[mine]) : -INFINITY;
     float score = 0.0f;
-    if (kByLogit && a.groups == 1 && a.renormalize != 0) top = Unordered(__shfl_sync(kFull, mine_key, 0));
+    if (kByLogit && a.groups == 1 && a.renormalize != 0) top = __shfl_sync(kFull, logit, 0);
     if (mine >= 0) {
-      const float logit = kByLogit ? Unordered(mine_key) : ToFloat(row[mine]);
       // The weights need no more than the divisions' two units in the last place.
       score = a.softmax != 0 ? __fdividef(expf(logit - top), total) : __fdividef(1.0f, 1.0f + expf(-logit));
       if (nan) score = __uint_as_float(0x7fc00000u);

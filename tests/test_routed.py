@@ -232,6 +232,21 @@ def test_route_gradient_against_differences():
 
 
 @gpu
+@pytest.mark.parametrize("experts", [8, 60, 128, 200, 512])
+def test_route_tells_neighbouring_logits_apart(experts):
+    """Logits that differ in their last bits only, some of them equal, of both signs: the order is by all bits, then
+    by index."""
+    g = torch.Generator().manual_seed(experts)
+    steps = torch.stack([torch.randperm(2 * experts, generator=g)[:experts] // 2 for _ in range(200)])
+    logits = (1 + steps.double() * 2.0 ** -23).float()
+    logits[1::2] *= -1
+    logits[::3, ::2] += 0.25                                # a few far from the others
+    r = routed.route(logits.cuda(), 8)
+    order = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :8]
+    assert torch.equal(r.experts.cpu().long(), order)
+
+
+@gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("tokens", [1, 100])
 def test_a_single_renormalised_choice_is_exact(tokens, score):
