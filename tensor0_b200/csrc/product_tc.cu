@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
   extern __shared__ unsigned char tc_raw[];
   __shared__ TcShared s;
   const uint32_t ring = (SharedAddress(tc_raw) + 1023u) & ~1023u;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int width = kKind == kProductTransposed ? a.inner : a.outer;
   const int tiles_n = (width + kWide - 1) / kWide;
   constexpr uint32_t kTmemColumns = 2 * kWide;
@@ -210,19 +210,20 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
           ok = BarrierWait(SharedAddress(&s.empty[stage]), (fill / Shape::kStages + 1) & 1, &s.failed);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         }
-        if (lane == 0) BarrierExpect(full, bytes);
+        const bool first = ElectOne();
+        if (first) BarrierExpect(full, bytes);
         __syncwarp();
         if constexpr (kKind == kProductWeightGrad) {
           if (load_a) {
             if (a.a_blocked != 0) {
-              if (lane == 0) LoadTile3(a_smem, &a.a, full, 0, t.begin + k0, t.m0 / 64);
+              if (first) LoadTile3(a_smem, &a.a, full, 0, t.begin + k0, t.m0 / 64);
             } else if (lane < a_blocks) {
               LoadTile2(a_smem + lane * kBlockBytes, &a.a, full, t.m0 + lane * 64, t.begin + k0);
             }
           }
           if (load_b) {
             if (a.b_blocked != 0) {
-              if (lane == 0) LoadTile3(b_smem, &a.b, full, 0, t.begin + k0, t.n0 / 64);
+              if (first) LoadTile3(b_smem, &a.b, full, 0, t.begin + k0, t.n0 / 64);
             } else if (lane < b_blocks) {
               LoadTile2(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, t.begin + k0);
             }
@@ -230,19 +231,19 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
         } else {
           if (load_a) {
             if (row_boxes == kTileRows / kRowBox) {
-              if (lane == 0) LoadTile2(a_smem, &a.a, full, k0, t.begin + t.m0);
+              if (first) LoadTile2(a_smem, &a.a, full, k0, t.begin + t.m0);
             } else if (lane < row_boxes) {
               LoadTile2(a_smem + lane * (kRowBox * kSwizzleRow), &a.a_few, full, k0, t.begin + t.m0 + lane * kRowBox);
             }
           }
           if constexpr (kKind == kProduct) {
             if (a.b_blocked != 0) {
-              if (lane == 0) LoadTile4(b_smem, &a.b, full, 0, k0, t.n0 / 64, t.e);
+              if (first) LoadTile4(b_smem, &a.b, full, 0, k0, t.n0 / 64, t.e);
             } else if (lane < b_blocks) {
               LoadTile3(b_smem + lane * kBlockBytes, &a.b, full, t.n0 + lane * 64, k0, t.e);
             }
           } else {
-            if (lane == 0) LoadTile3(b_smem, &a.b, full, k0, t.n0, t.e);
+            if (first) LoadTile3(b_smem, &a.b, full, k0, t.n0, t.e);
           }
         }
       }
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
       BarrierWait(SharedAddress(&s.full[f % Shape::kStages]), (f / Shape::kStages) & 1, nullptr);
     }
   } else if (warp == 1) {
-    // Matrix instructions, issued by lane 0.
+    // Matrix instructions, issued by one lane.
     constexpr uint32_t a_major = kKind == kProductWeightGrad ? 1u : 0u, b_major = kKind == kProductTransposed ? 0u : 1u;
     const uint32_t format = a.bf16 != 0 ? 1u : 0u;
     const uint32_t idesc = (1u << 4) | (format << 7) | (format << 10) | (a_major << 15) | (b_major << 16) |
@@ -274,12 +275,14 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         const uint32_t a_smem = ring + stage * Shape::kStageBytes, b_smem = a_smem + kABytes;
         if constexpr (kGather) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        // The last slice: what is left of the sum, in steps of 16.
+        const int deep = (kKind == kProductWeightGrad ? t.count : kKind == kProduct ? a.inner : a.outer) - k * kDeep;
+        const int steps = min(kDeep, deep + 15) / 16;
         if constexpr (kKind == kProductWeightGrad) {
-          const int valid = t.count - k * kDeep;
-          if (valid < kDeep) {   // rows of the next expert: zero, in every column block of both operands
+          if (steps * 16 > deep) {   // rows of the next expert: zero, in every column block of both operands
             for (int block = 0; block < 2 + kWide / 64; ++block) {
-              const uint32_t to = a_smem + (block + 1) * kBlockBytes;
-              for (uint32_t at = to - (kDeep - valid) * kSwizzleRow + lane * 16; at < to; at += 512) {
+              const uint32_t to = a_smem + block * kBlockBytes + steps * (16 * kSwizzleRow);
+              for (uint32_t at = to - (steps * 16 - deep) * kSwizzleRow + lane * 16; at < to; at += 512) {
                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
               }
             }
@@ -288,14 +291,20 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
           }
         }
         TmemFenceAfter();
-        if (lane == 0) {
+        if (ElectOne()) {
+          const uint64_t left = a_major ? WideMajor(a_smem, kBlockBytes) : DeepMajor(a_smem);
+          const uint64_t right = b_major ? WideMajor(b_smem, kBlockBytes) : DeepMajor(b_smem);
+          constexpr uint32_t left_step = (a_major ? 16 * kSwizzleRow : 32) >> 4, right_step = (b_major ? 16 * kSwizzleRow : 32) >> 4;
+          if (steps == kDeep / 16) {
 #pragma unroll
-          for (int step = 0; step < kDeep / 16; ++step) {
-            const uint64_t left = a_major ? WideMajor(a_smem + step * 16 * kSwizzleRow, kBlockBytes)
-                                          : DeepMajor(a_smem + step * 32);
-            const uint64_t right = b_major ? WideMajor(b_smem + step * 16 * kSwizzleRow, kBlockBytes)
-                                           : DeepMajor(b_smem + step * 32);
-            MmaHalf(accumulator, left, right, idesc, k == 0 && step == 0 ? 0u : 1u);
+            for (int step = 0; step < kDeep / 16; ++step) {
+              MmaHalf(accumulator, left + step * left_step, right + step * right_step, idesc, k == 0 && step == 0 ? 0u : 1u);
+            }
+          } else {
+#pragma unroll 1
+            for (int step = 0; step < steps; ++step) {
+              MmaHalf(accumulator, left + step * left_step, right + step * right_step, idesc, k == 0 && step == 0 ? 0u : 1u);
+            }
           }
           MmaCommit(SharedAddress(&s.empty[stage]));
           if (k == slices - 1) MmaCommit(SharedAddress(&s.done[buffer]));
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
       ++turn;
     }
     if (!ok) {
-      if (lane == 0) MmaCommit(SharedAddress(&s.drain));
+      if (ElectOne()) MmaCommit(SharedAddress(&s.drain));
       BarrierWait(SharedAddress(&s.drain), 0, nullptr);
     }
   } else if (warp < 6) {

@@ -12,6 +12,15 @@ __device__ __forceinline__ uint32_t SharedAddress(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// True in one lane of a whole warp, always the same one.  (Matrix instructions
+// under a test of the lane number instead took up to 10 % longer per product:
+// 7.1 us instead of 6.1 for a small one, 2048 x 2048 weights 228 instead of 218.)
+__device__ __forceinline__ bool ElectOne() {
+  uint32_t chosen;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(chosen));
+  return chosen != 0;
+}
+
 __device__ __forceinline__ void BarrierInit(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
