@@ -20,14 +20,16 @@
 // matrix warp zeroes them in shared memory, in both operands, so that a value
 // that is not finite stays with its own expert.
 //
-// Measured, bf16: 32768 rows of 64 experts, 1024 x 2048, 138 us (1.0 PFLOP/s,
-// 0.62 of the matrix rate; every second expert's last tile is half empty); of 32
-// experts at 2048 x 2048 230 us (1.2); that weight gradient 255 us, with gathered
-// rows 330.  9222 rows of 40 experts at 1000 x 1416 f16 49 us, where reading the
+// Measured, bf16: 32768 rows of 64 experts, 1024 x 2048, 133 us (1.0 PFLOP/s,
+// 0.64 of the matrix rate; every second expert's last tile is half empty); of 32
+// experts at 2048 x 2048 220 us (1.25); that weight gradient 250 us, with gathered
+// rows 304.  9222 rows of 40 experts at 1000 x 1416 f16 48 us, where reading the
 // weights takes 17.  What bounds: the slices' latency against four stages, and at
 // few rows per expert the weights' bytes.
-// Two blocks sharing 256 x 256 tiles (cta_group::2) were slower: 265 us where
-// this takes 232, for the tiles' empty halves and the blocks' handshakes.
+// Slower: two blocks sharing 256 x 256 tiles (cta_group::2), 265 us where this
+// took 232, for the tiles' empty halves and the blocks' handshakes; eight storing
+// warps, 34 us instead of 30 for the weight gradient of 64 rows of 32 experts,
+// 2048 x 1024, and no gain for large ones.
 #include <algorithm>
 
 #include "engine.h"
@@ -532,10 +534,14 @@ void ByWidth(const ProductArgs& p, bool bf16, cudaStream_t stream) {
   // The widest tile that still gives every other multiprocessor one: what a
   // block brings per slice grows with the width, and narrow tiles bring the
   // rows of x more often (512 rows of 64 experts, 1024 x 1024: 27 us with 256
-  // columns, 32 with 128, 48 with 64; one row of 8 experts, 512 x 512: 8.1, 7.1
-  // and 6.7 us).
-  if (2 * tiles(256) >= sms) launch(std::integral_constant<int, 256>{});
-  else if (2 * tiles(128) >= sms) launch(std::integral_constant<int, 128>{});
+  // columns, 28 with 128, 33 with 64; one row of two experts, 512 x 512: 6.4, 5.4
+  // and 4.9 us).  Partial row tiles count as half of one here (3000 rows of 24
+  // experts, 768 x 384: 7.3 us with 128 columns, 8.7 with 256).
+  const int64_t used = std::min<int64_t>(p.experts, p.entries);
+  const int64_t likely = kKind == kProductWeightGrad ? row_tiles : std::max(used, p.entries / kTileRows + used / 2);
+  const auto enough = [&](int wide) { return 2 * likely * ((width + wide - 1) / wide) >= sms; };
+  if (enough(256)) launch(std::integral_constant<int, 256>{});
+  else if (enough(128)) launch(std::integral_constant<int, 128>{});
   else launch(std::integral_constant<int, 64>{});
 }
 
