@@ -5,25 +5,28 @@
 // tiles.  Warp 0 loads 64-deep slices into a ring of shared-memory stages by
 // TMA.  One thread of warp 1 issues the matrix instructions into one of two
 // accumulators in tensor memory, and warps 2 to 5 round and store the other one
-// meanwhile.  Where rows are gathered, warps 6 to 9 copy them by their indices
+// meanwhile.  Where rows are gathered, warps 6 to 13 copy them by their indices
 // with 16-byte asynchronous copies, straight from the token rows: no ordered
 // copy of the input is made.  (TMA's own four-row gather was measured at about
 // 100 cycles an instruction, 512 bytes each: 1.8 us a slice against 0.28 us of
-// matrix instructions.)
+// matrix instructions.  Four copying warps took 348 us for a weight gradient with
+// gathered y where eight take 303, and one microsecond longer for small calls;
+// sixteen were slower again.)
 //
 //   product:     A = rows of x (deep-major), B = W[e] as it lies (wide-major)
 //   transposed:  A = rows of x (deep-major), B = W[e]^T: W[e] as it lies (deep-major)
 //   weight grad: A = x^T, B = y: rows are the deep axis, both as they lie (wide-major)
 //
 // A tile's rows past its expert's last are computed from whatever lies in
-// shared memory and not stored (experts with few rows load few).  In the weight gradient they would enter the sum: the
-// matrix warp zeroes them in shared memory, in both operands, so that a value
-// that is not finite stays with its own expert.
+// shared memory and not stored (experts with few rows load few).  In the weight
+// gradient they would enter the sum: the matrix warp zeroes them in shared
+// memory, in both operands, so that a value that is not finite stays with its
+// own expert.
 //
 // Measured, bf16: 32768 rows of 64 experts, 1024 x 2048, 133 us (1.0 PFLOP/s,
 // 0.64 of the matrix rate; every second expert's last tile is half empty); of 32
 // experts at 2048 x 2048 220 us (1.25); that weight gradient 250 us, with gathered
-// rows 304.  9222 rows of 40 experts at 1000 x 1416 f16 48 us, where reading the
+// rows 275 (x) or 303 (y).  9222 rows of 40 experts at 1000 x 1416 f16 48 us, where reading the
 // weights takes 17.  What bounds: the slices' latency against four stages, and at
 // few rows per expert the weights' bytes.
 // Slower: two blocks sharing 256 x 256 tiles (cta_group::2), 265 us where this
@@ -43,7 +46,8 @@ namespace t0b {
 namespace {
 
 constexpr int kTileRows = 128, kDeep = 64, kRowBox = 32;   // kRowBox: rows of x that one copy brings
-constexpr int kTcThreads = 192, kGatherThreads = 128;      // roles; copying threads where rows are gathered
+constexpr int kTcThreads = 192, kGatherThreads = 256;      // roles; copying threads where rows are gathered
+constexpr int kGatherRows = kGatherThreads / 8;            // rows that they copy at a time
 constexpr uint32_t kSwizzleRow = 128;                      // bytes of 64 16-bit values
 constexpr uint32_t kABytes = kTileRows * kSwizzleRow;      // one stage of A
 constexpr uint32_t kBlockBytes = kDeep * kSwizzleRow;      // 64 x 64 values
@@ -394,7 +398,7 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
     }
   } else if constexpr (kGather) {
     // Gathered rows: eight threads copy 128 bytes of a row, a thread the same
-    // chunk of rows r0, r0 + 16, ...  A thread's arrival at the stage's barrier
+    // chunk of rows r0, r0 + 32, ...  A thread's arrival at the stage's barrier
     // follows its copies by itself; the matrix warp then orders them before the
     // tensor cores' reads.
     const int g = tid - kTcThreads, c = g & 7, r0 = g >> 3;
@@ -404,16 +408,18 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
       const TcTile t = walk.At(tile);
       const int slices = walk.Slices(t), last = t.begin + t.count - 1;
       const int valid = t.count - t.m0;   // rows of the tile (products)
-      const uint16_t* source[8];          // where they lie
-      int next[4];                 // entries of the next slice's rows (weight gradient), used a slice later
+      const uint16_t* source[kTileRows / kGatherRows];   // where they lie
+      int next[kDeep / kGatherRows];   // entries of the next slice's rows (weight gradient), used a slice later
       auto slice_rows = [&](int k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) next[i] = a.rows[min(t.begin + k * kDeep + r0 + 16 * i, last)];
+        for (int i = 0; i < kDeep / kGatherRows; ++i) {
+          next[i] = a.rows[min(t.begin + k * kDeep + r0 + kGatherRows * i, last)];
+        }
       };
       if constexpr (kKind != kProductWeightGrad) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int64_t row = a.rows[min(t.begin + t.m0 + r0 + 16 * i, last)] / a.top_k;
+        for (int i = 0; i < kTileRows / kGatherRows; ++i) {
+          const int64_t row = a.rows[min(t.begin + t.m0 + r0 + kGatherRows * i, last)] / a.top_k;
           source[i] = a.a_data + (row >= 0 && row < a.a_rows ? row : 0) * a.a_stride + c * 8;
         }
       } else if (slices > 0) {
@@ -430,22 +436,28 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
           const int deep = kKind == kProduct ? a.inner : a.outer;
           const bool inside = k * kDeep + c * 8 < deep;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (r0 + 16 * i < valid) CopyChunk(a_smem, r0 + 16 * i, c, inside ? source[i] + k * kDeep : a.a_data, inside);
+          for (int i = 0; i < kTileRows / kGatherRows; ++i) {
+            const int r = r0 + kGatherRows * i;
+            if (r < valid) CopyChunk(a_smem, r, c, inside ? source[i] + k * kDeep : a.a_data, inside);
           }
         } else {
-          int64_t row[4];
+          int64_t row[kDeep / kGatherRows];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) row[i] = next[i] / a.top_k;
+          for (int i = 0; i < kDeep / kGatherRows; ++i) row[i] = next[i] / a.top_k;
           if (k + 1 < slices) slice_rows(k + 1);
           auto copy = [&](uint32_t tile_smem, const uint16_t* data, int64_t rows, int64_t stride, int column, int columns,
                           int blocks) {
-            for (int block = 0; block < blocks; ++block) {
-              const int at = column + block * 64 + c * 8;
+            const uint16_t* from[kDeep / kGatherRows];   // null: no such row
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const bool inside = at < columns && row[i] >= 0 && row[i] < rows;
-                CopyChunk(tile_smem + block * kBlockBytes, r0 + 16 * i, c, inside ? data + row[i] * stride + at : data,
+            for (int i = 0; i < kDeep / kGatherRows; ++i) {
+              from[i] = row[i] >= 0 && row[i] < rows ? data + row[i] * stride + column + c * 8 : nullptr;
+            }
+            for (int block = 0; block < blocks; ++block) {
+              const bool in_row = column + block * 64 + c * 8 < columns;
+#pragma unroll
+              for (int i = 0; i < kDeep / kGatherRows; ++i) {
+                const bool inside = in_row && from[i] != nullptr;
+                CopyChunk(tile_smem + block * kBlockBytes, r0 + kGatherRows * i, c, inside ? from[i] + block * 64 : data,
                           inside);
               }
             }
