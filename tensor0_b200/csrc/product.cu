@@ -110,8 +110,11 @@ __global__ void __launch_bounds__(kGenThreads) GeneralProduct(ProductArgs a, int
   }
 }
 
-// A warp sums 256 columns (blockIdx.y) of one token; memory bound, each row
-// read once, four rows in flight.
+// A warp sums 256 columns (blockIdx.y) of one token in 32 bits; memory bound,
+// each row read once, four rows in flight.  The rows come rounded to 16 bits, so
+// that they take half the traffic: their errors and the result's together are
+// about 1.4 times those of one rounding, where 32-bit rows would move 268 MB more
+// (41 us of copy bandwidth) for 8192 tokens of 4 rows of 2048.
 template <typename T, bool Vector>
 __global__ void __launch_bounds__(256) RoutedSum(RoutedSumArgs a) {
   LetNextStart();

@@ -395,6 +395,35 @@ def test_a_row_that_is_not_finite_stays_its_own():
 
 
 @gpu
+@pytest.mark.parametrize("gather", [(False, False), (True, False), (False, True)])
+@pytest.mark.parametrize("inner,outer", [(128, 256), (72, 136)])
+def test_weight_gradients_end_with_their_experts_rows(gather, inner, outer):
+    """Row counts around the steps and slices of the sum, every second expert's rows not finite; whole numbers."""
+    counts = [1, 3, 15, 2, 16, 5, 17, 1, 33, 40, 47, 48, 49, 9, 63, 64, 65, 1, 112, 7, 127, 128, 129, 30]
+    offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    total, expert = int(offsets[-1]), np.repeat(np.arange(len(counts)), counts)
+    g = torch.Generator().manual_seed(13)
+    rows = torch.randperm(total, generator=g)            # one slot: an entry is a token
+    positions = torch.argsort(rows).int()
+    r = routed.Routing(*(t.cuda() for t in (torch.from_numpy(expert)[positions.long()].int()[:, None],
+                                            torch.ones(total, 1), rows.int(), positions[:, None],
+                                            torch.from_numpy(offsets))))
+    x = torch.randint(-3, 4, (total, inner), generator=g).bfloat16()
+    y = torch.randint(-3, 4, (total, outer), generator=g).bfloat16()
+    expected = np.zeros((len(counts), inner, outer))
+    for e in range(0, len(counts), 2):
+        expected[e] = wide(x[expert == e]).T @ wide(y[expert == e])
+    x[expert % 2 == 1], y[expert % 2 == 1] = math.nan, math.inf
+
+    def by_token(ordered):
+        return ordered[positions.long()]
+    got = routed.routed_weight_grad((by_token(x) if gather[0] else x).cuda(), (by_token(y) if gather[1] else y).cuda(), r,
+                                    gather_x=gather[0], gather_y=gather[1])
+    assert torch.equal(got[::2].cpu(), torch.from_numpy(expected[::2]).bfloat16())
+    assert not torch.isfinite(got[1::2]).any()
+
+
+@gpu
 def test_products_take_strided_rows_and_repeat_their_bits():
     host, r = make_routing(200, 7, 3, 12)
     store = torch.randn(200, 160).half().cuda()
