@@ -42,6 +42,7 @@ sys.path.insert(0, str(ROOT))
 
 METRIC = "block-permute/accumulate HBM GB/s"
 UNIT = "GB/s"
+NO_REFERENCE = "the reference's CPU library (oracle/_ref) is not built: its sources are not present"
 
 
 def parse():
@@ -130,6 +131,10 @@ def run_reference(args, rank: int):
     """The reference's CPU executors on the same workload as the GPU arm (full
     size), on all host cores; rank 0 only."""
     if rank != 0:
+        return
+    from oracle import ref
+    if not ref.LIBRARY.exists():
+        print(json.dumps({"impl": "reference", "unavailable": NO_REFERENCE}), flush=True)
         return
     threads = os.cpu_count() or 1
     value, ms, sample, n = cpu_reference_steps(args.dtype, args.steps, args.warmup, threads, args.scale)
@@ -771,9 +776,13 @@ def main():
 
     cpu = None
     if not args.no_cpu_baseline:
+        from oracle import ref
         threads = os.cpu_count() or 1
-        value_cpu, ms_cpu, sample, _ = cpu_reference_steps(args.dtype, 3, 1, threads, SAMPLE_SCALE)
-        cpu = {"value": round(value_cpu, 3), "unit": UNIT, "cores": threads, "kind": "reference", "sample": sample}
+        if not ref.LIBRARY.exists():
+            cpu = {"unavailable": NO_REFERENCE}
+        else:
+            value_cpu, ms_cpu, sample, _ = cpu_reference_steps(args.dtype, 3, 1, threads, SAMPLE_SCALE)
+            cpu = {"value": round(value_cpu, 3), "unit": UNIT, "cores": threads, "kind": "reference", "sample": sample}
 
     line = {
         "metric": METRIC, "value": round(value, 3), "unit": UNIT, "n_gpus": 1, "steps": args.steps,
