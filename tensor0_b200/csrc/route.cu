@@ -8,7 +8,8 @@
 //   stay, then the top_k best c of what stays; ties go to the lowest index.
 //   w = scale * s / (sum of the chosen s + 1e-20), or scale * s.
 // A logit of -inf or NaN, and a masked token, take no expert (index -1,
-// weight 0).  Under softmax a NaN or +inf logit makes the row's weights NaN.
+// weight 0).  Under softmax a NaN or +inf logit makes the row's weights NaN,
+// whichever experts it leaves to choose from.
 //
 // One warp holds a token: lane l has the V experts from l * V on.  Bound by
 // instructions, not by memory, so nothing is done for all experts where it can
@@ -299,6 +300,18 @@ __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, 
       for (int j = 0; j < V; ++j) c[j] = x[j];
     } else {
       if (a.softmax != 0) {
+        if (nan || top == INFINITY) {
+          // No scores: the choice goes by those without the NaN logits, or by
+          // their limits, equal shares for +inf and nothing for the others.
+          nan = true;
+          const bool infinite = top == INFINITY;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (!(x[j] > -INFINITY)) x[j] = -INFINITY;
+            else if (infinite) x[j] = x[j] == INFINITY ? 0.0f : -1e30f;
+          }
+          if (infinite) top = 0.0f;
+        }
         // Summed in 64 bits and rounded once: the choice, which goes by these
         // scores, does not depend on the order of the terms.
         double sum = 0.0;

@@ -1,0 +1,55 @@
+"""Routed operators at inputs that are not finite, at the limits that they accept, on strided operands, and from more
+than one thread.  Tolerances are those of ``test_routed``: they follow from the arithmetic."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tensor0_b200 import routed
+from test_routed import TYPES, plain_choice, wide
+
+gpu = pytest.mark.gpu
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Router
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [6, 300])                  # one block, and several
+@pytest.mark.parametrize("experts, groups, top_groups, best, bias",
+                         [(16, 1, 1, 1, True), (40, 1, 1, 2, False), (64, 4, 2, 1, True), (256, 8, 4, 2, True)])
+def test_a_choice_by_scores_surfaces_numbers_that_are_not(experts, groups, top_groups, best, bias, tokens, dtype):
+    """A NaN logit takes no expert and the others stay; +inf takes the score 1, shared if there are several.  The
+    weights and the gradient of such a row are NaN, other rows are as without it."""
+    g = torch.Generator().manual_seed(experts + tokens)
+    logits = torch.randn(tokens, experts, generator=g).to(TYPES[dtype])
+    b = 0.3 * torch.randn(experts, generator=g) if bias else None
+    plain = {"groups": groups, "top_groups": top_groups, "group_best": best, "bias": None if b is None else b.cuda()}
+    fine = routed.route(logits.cuda(), 4, **plain)
+    logits[0, 5] = math.nan
+    logits[1, 5] = math.inf
+    logits[2, 3], logits[2, 7] = math.nan, math.inf
+    logits[3, 2] = logits[3, 11] = math.inf
+    logits[4] = math.nan
+    r = routed.route(logits.cuda(), 4, **plain)
+    # The definition on the same rows: without the NaN logits, and at +inf the scores' limits.
+    x = logits[:5].double().numpy()
+    infinite = np.isinf(x).any(1, keepdims=True)
+    limit = np.where(infinite, np.where(np.isinf(x), 0.0, -1e30), x)
+    limit[np.isnan(x)] = -np.inf
+    with np.errstate(all="ignore"):
+        chosen, scores = plain_choice(limit, 4, groups, top_groups, best, True, None if b is None else wide(b), None)
+    got = r.experts[:5].cpu().numpy()
+    for t in np.unique(np.nonzero(got != chosen)[0]):         # closer than 32-bit choice values are rounded
+        value = scores[t] + (0 if b is None else wide(b))
+        assert (got[t] >= 0).all() and (chosen[t] >= 0).all(), t
+        assert np.max(np.abs(np.sort(value[got[t]]) - np.sort(value[chosen[t]]))) < 2.0 ** -20, t
+    assert (chosen[:4] >= 0).all() and (chosen[4] < 0).all()
+    assert torch.isnan(r.weights[:4]).all() and (r.weights[4] == 0).all()
+    assert torch.equal(r.experts[5:], fine.experts[5:]) and torch.equal(r.weights[5:], fine.weights[5:])
+    grad = routed.route_backward(logits.cuda(), r, torch.ones(tokens, 4).cuda())
+    assert torch.isnan(grad[:4]).any(1).all() and (grad[4] == 0).all() and torch.isfinite(grad[5:]).all()
