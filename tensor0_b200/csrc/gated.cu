@@ -143,6 +143,8 @@ struct RawCodes {
 };
 
 // A group's units per value and its scale, from the largest magnitude's bits.
+// An infinity's group has the scale NaN: an infinite scale would make -inf of a
+// code below 0, which is what a value that has no code may leave.
 struct GroupScale {
   float per_unit, scale;
   __device__ __forceinline__ explicit GroupScale(uint32_t bits) {
@@ -150,6 +152,7 @@ struct GroupScale {
     const bool none = largest < kSmallest;
     per_unit = none ? 0.0f : __frcp_rn(largest) * 127.0f;
     scale = none ? 0.0f : largest * (1.0f / 127.0f);
+    if (bits >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
   }
 };
 

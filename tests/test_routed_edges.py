@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tensor0_b200 import routed
-from test_routed import TYPES, plain_choice, wide
+from test_routed import HALF, TYPES, plain_choice, wide
 
 gpu = pytest.mark.gpu
 
@@ -53,3 +53,29 @@ def test_a_choice_by_scores_surfaces_numbers_that_are_not(experts, groups, top_g
     assert torch.equal(r.experts[5:], fine.experts[5:]) and torch.equal(r.weights[5:], fine.weights[5:])
     grad = routed.route_backward(logits.cuda(), r, torch.ones(tokens, 4).cuda())
     assert torch.isnan(grad[:4]).any(1).all() and (grad[4] == 0).all() and torch.isfinite(grad[5:]).all()
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Gated activation and its checkpoint
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("width, group", [(64, 32), (128, 64), (256, 128), (61, 32), (77, 64), (130, 128)])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_checkpoint_of_an_infinity_is_not_a_number(value, width, group, dtype):
+    """The whole group of an infinite value loads as NaN, and its gradient is NaN: no infinity of the other sign."""
+    h = torch.randn(3, 2 * width, generator=torch.Generator().manual_seed(width)).to(HALF[dtype][0])
+    gate, up = 5, width + width - 1                       # one in the first group of the gate, one in the last of the up
+    h[1, gate] = h[2, up] = value
+    _, kept = routed.gated_save(h.cuda(), group=group)
+    column = np.arange(2 * width)
+    of = np.where(column < width, column // group, 1000 + (column - width) // group)
+    values = wide(routed.checkpoint_load(kept))
+    for row, at in ((1, gate), (2, up)):
+        assert np.array_equal(np.isnan(values[row]), of == of[at])
+        assert np.isfinite(values[row][of != of[at]]).all()
+    assert np.isfinite(values[0]).all()
+    h_grad, a, weights_grad = routed.gated_backward(kept, torch.ones(3, width).to(HALF[dtype][0]).cuda())
+    assert torch.isnan(h_grad[1, gate]) and torch.isnan(h_grad[2, up - width]) and torch.isnan(a[2, up - width])
+    assert torch.isnan(weights_grad[1:]).all() and torch.isfinite(weights_grad[0]) and torch.isfinite(h_grad[0]).all()
