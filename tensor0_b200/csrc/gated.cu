@@ -31,14 +31,24 @@ constexpr int kGatedThreads = 256;
 constexpr const char* kLaunch = "gated activation launch";
 constexpr float kSmallest = 0x1p-100f;   // 127 / m and m / 127 stay normal numbers above it
 
-// 1 / (1 + exp(-g)) in four instructions, off by a few units in the last place
-// of 1 + exp(-g).  (Without .ftz each of the two special functions takes a
-// comparison and a scaling more; what they flush is far below the result's type.)
+// 1 / (1 + exp(-g)), off by a few units in the last place of 1 + exp(-g).
+// Without .ftz each of the two special functions takes a comparison and a scaling
+// more.  What they flush, below 2^-126, is far below F16 (four instructions).  BF16
+// reaches down to 2^-133, which silu passes at g = -97 only: there the sum is held
+// as 2^-15 (1 + exp(-g)), which is below 2^126 down to g = -97.7, and the reciprocal
+// is scaled back by a product that keeps subnormal numbers.
+template <typename T>
 __device__ __forceinline__ float Sigmoid(float g) {
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return r;
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
+  } else {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fmaf(g, -1.4426950408889634f, -15.0f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0x1p-15f + e));
+    return r * 0x1p-15f;
+  }
 }
 
 // Row p's routing weight; false if the row belongs to no expert.
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 4) GatedSave(Gated
       raw_u.Values(u);
       // A row that is not present is zeros, whose activation is zero.
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = (weight * g[i]) * Sigmoid(g[i]) * u[i];
+      for (int i = 0; i < 8; ++i) out[i] = (weight * g[i]) * Sigmoid<T>(g[i]) * u[i];
       StoreRow<T, Vector>(out_row, left, lane, out);
       if (a.codes != nullptr) {   // null: the activation alone
         StoreCodes<T, Vector, kShift>(raw_g, g, left, lane, codes, scales);
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(kGatedThreads, Vector ? 0 : 3) GatedBackward(G
       if (Vector && base + 256 < a.width) fetch(base + 256);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float s = Sigmoid(g[i]), silu = g[i] * s;
+        const float s = Sigmoid<T>(g[i]), silu = g[i] * s;
         const float wda = weight * da[i], silu_u = silu * u[i];
         dg[i] = wda * u[i] * fmaf(silu, 1.0f - s, s);
         du[i] = wda * silu;

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tensor0_b200 import routed
-from test_routed import HALF, TYPES, plain_choice, wide
+from test_routed import HALF, TYPES, near, plain_choice, wide
 
 gpu = pytest.mark.gpu
 
@@ -79,3 +79,26 @@ def test_checkpoint_of_an_infinity_is_not_a_number(value, width, group, dtype):
     h_grad, a, weights_grad = routed.gated_backward(kept, torch.ones(3, width).to(HALF[dtype][0]).cuda())
     assert torch.isnan(h_grad[1, gate]) and torch.isnan(h_grad[2, up - width]) and torch.isnan(a[2, up - width])
     assert torch.isnan(weights_grad[1:]).all() and torch.isfinite(weights_grad[0]) and torch.isfinite(h_grad[0]).all()
+
+
+@gpu
+def test_gates_far_below_zero_keep_bf16_range():
+    """silu(-88) is -5e-37, a normal number of BF16: down to the smallest subnormal, 2^-133."""
+    gates = -torch.linspace(80, 99, 96).bfloat16()
+    h = torch.cat([gates, torch.ones(96).bfloat16()])[None].cuda()
+    a, kept = routed.gated_save(h, group=32)
+    g = wide(h)[0, :96]
+    silu = g / (1 + np.exp(-g))
+    # exp's argument is rounded: 1.2 |gate| + 2 units of 2^-23; the sigmoid may be a subnormal of 2^-149.
+    slack = 125 * 2.0 ** -23
+    near(a[0], silu, (1.01 * 2.0 ** -8 + slack) * np.abs(silu) + 2.0 ** -134 + 100 * 2.0 ** -149, "activation")
+    assert float(a[0, 0]) < 0
+    da = torch.ones(1, 96).bfloat16().cuda()
+    h_grad, again, weights_grad = routed.gated_backward(kept, da)
+    x = wide(routed.checkpoint_load(kept))[0]
+    g, u = x[:96], x[96:]
+    s = 1 / (1 + np.exp(-g))
+    near(again[0], g * s * u, (1.01 * 2.0 ** -8 + slack) * np.abs(g * s * u) + 2.0 ** -134 + 100 * 2.0 ** -149, "again")
+    both = np.concatenate([u * (s + g * s * (1 - s)), g * s])
+    size = np.concatenate([np.abs(u) * (s + np.abs(g * s)), np.abs(g * s)])
+    near(h_grad[0], both, 1.01 * 2.0 ** -8 * np.abs(both) + slack * size + 2.0 ** -134 + 200 * 2.0 ** -149, "gradient")
