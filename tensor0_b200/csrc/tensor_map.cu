@@ -1,6 +1,7 @@
 #include "tensor_map.h"
 
 #include <stdexcept>
+#include <string>
 
 #include "engine.h"
 
@@ -30,10 +31,21 @@ CUtensorMap Encode(CUtensorMapDataType type, const void* data, int rank, const c
                    const cuuint64_t* strides, const cuuint32_t* boxes) {
   const cuuint32_t steps[4] = {1, 1, 1, 1};
   CUtensorMap map;
-  const CUresult status = Encoder()(&map, type, rank, const_cast<void*>(data), sizes, strides, boxes, steps,
-                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (status != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed");
+  const auto encode = [&] {
+    return Encoder()(&map, type, rank, const_cast<void*>(data), sizes, strides, boxes, steps,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult status = encode();
+  if (status == CUDA_ERROR_INVALID_CONTEXT || status == CUDA_ERROR_NOT_INITIALIZED) {
+    // A thread that has not used the device: unlike the runtime's functions, the
+    // driver's do not make the device's context current themselves.
+    int device = 0;
+    Check(cudaGetDevice(&device), "current device");
+    Check(cudaSetDevice(device), "device context");
+    status = encode();
+  }
+  if (status != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed with error " + std::to_string(status));
   return map;
 }
 

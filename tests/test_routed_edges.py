@@ -2,13 +2,14 @@
 than one thread.  Tolerances are those of ``test_routed``: they follow from the arithmetic."""
 
 import math
+import threading
 
 import numpy as np
 import pytest
 import torch
 
 from tensor0_b200 import routed
-from test_routed import HALF, TYPES, near, plain_choice, wide
+from test_routed import HALF, TYPES, make_routing, near, plain_choice, wide
 
 gpu = pytest.mark.gpu
 
@@ -102,3 +103,67 @@ def test_gates_far_below_zero_keep_bf16_range():
     both = np.concatenate([u * (s + g * s * (1 - s)), g * s])
     size = np.concatenate([np.abs(u) * (s + np.abs(g * s)), np.abs(g * s)])
     near(h_grad[0], both, 1.01 * 2.0 ** -8 * np.abs(both) + slack * size + 2.0 ** -134 + 200 * 2.0 ** -149, "gradient")
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Threads
+
+
+@gpu
+@pytest.mark.parametrize("name", ["routed_matmul", "routed_weight_grad", "routed_matvec"])
+def test_a_threads_first_call(name):
+    """A thread that has not used the device yet, as autograd's are: the same result as on the main thread."""
+    _, r = make_routing(12, 4, 2, 17)
+    x, w = torch.randn(12, 64).bfloat16().cuda(), torch.randn(4, 64, 32).bfloat16().cuda()
+    y = torch.randn(24, 32).bfloat16().cuda()
+    call = {"routed_matmul": lambda: routed.routed_matmul(x, w, r, gather=True),
+            "routed_weight_grad": lambda: routed.routed_weight_grad(x, y, r, gather_x=True),
+            "routed_matvec": lambda: routed.routed_matvec(x, routed.Int4Weights(*four), r, gather=True)}[name]
+    four = routed.pack_int4(w, 32)
+    expected = call()
+    found = []
+
+    def work():
+        try:
+            found.append(call())
+        except Exception as error:
+            found.append(error)
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    assert isinstance(found[0], torch.Tensor), found[0]
+    assert torch.equal(found[0], expected)
+
+
+class Product(torch.autograd.Function):
+    """How a user joins the operators to autograd: each backward operator in its own Function."""
+    @staticmethod
+    def forward(ctx, x, w, *routing):
+        r = routed.Routing(*routing)
+        ctx.save_for_backward(x, w, *routing)
+        return routed.routed_sum(routed.routed_matmul(x, w, r, gather=True), r)
+
+    @staticmethod
+    def backward(ctx, y_grad):
+        x, w, *routing = ctx.saved_tensors
+        r = routed.Routing(*routing)
+        rows = routed.routed_matmul(y_grad, w, r, gather=True, transpose=True)
+        return routed.routed_sum(rows, r), routed.routed_weight_grad(x, y_grad, r, gather_x=True, gather_y=True), *[None] * 5
+
+
+@gpu
+def test_operators_inside_a_function():
+    host, r = make_routing(40, 4, 2, 21)
+    g = torch.Generator().manual_seed(2)
+    x = torch.randint(-2, 3, (40, 64), generator=g).bfloat16().cuda().requires_grad_()
+    w = torch.randint(-2, 3, (4, 64, 8), generator=g).bfloat16().cuda().requires_grad_()
+    y = Product.apply(x, w, *r)
+    y.backward(torch.ones_like(y))
+    xd, wd = x.detach().double().cpu().requires_grad_(), w.detach().double().cpu().requires_grad_()
+    chosen = torch.from_numpy(host[0]).long()
+    expected = torch.einsum("ti,tkio->to", xd, wd[chosen])
+    expected.backward(torch.ones_like(expected))
+    # sums of whole numbers: exact up to 256, beyond that one rounding of each row and of the sum
+    assert torch.allclose(y.detach().double().cpu(), expected.detach(), rtol=2 * 2.0 ** -8, atol=2.0)
+    assert torch.allclose(x.grad.double().cpu(), xd.grad, rtol=2 * 2.0 ** -8, atol=0.5)
+    assert torch.allclose(w.grad.double().cpu(), wd.grad, rtol=2.0 ** -8, atol=0.5)
