@@ -7,6 +7,7 @@
 #include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 #include <utility>
 
 #include "engine.h"
@@ -146,14 +147,19 @@ inline bool BriefGrid(int64_t blocks) { return blocks <= 2 * RoutedSmCount(); }
 
 // Lets kernel `kKernel` use `bytes` of dynamic shared memory on the current
 // device; asked for once per device and size, since the call costs as much as
-// a launch's share of a small operator.
+// a launch's share of a small operator.  Under a lock, so that the limit only
+// grows: another thread's smaller size neither takes it back nor is recorded
+// over a larger one.
 template <auto kKernel>
 void AllowShared(int bytes) {
   static std::atomic<int> allowed[kMaxDevices];
+  static std::mutex setting;
   const int device = CurrentDevice();
-  if (bytes <= 48 * 1024 || allowed[device].load(std::memory_order_relaxed) >= bytes) return;
+  if (bytes <= 48 * 1024 || allowed[device].load(std::memory_order_acquire) >= bytes) return;
+  const std::lock_guard<std::mutex> lock(setting);
+  if (allowed[device].load(std::memory_order_relaxed) >= bytes) return;
   Check(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "kernel shared memory");
-  allowed[device].store(bytes, std::memory_order_relaxed);
+  allowed[device].store(bytes, std::memory_order_release);
 }
 
 }  // namespace t0b

@@ -2,13 +2,14 @@
 than one thread.  Tolerances are those of ``test_routed``: they follow from the arithmetic."""
 
 import math
+import subprocess
 import threading
 
 import numpy as np
 import pytest
 import torch
 
-from tensor0_b200 import routed
+from tensor0_b200 import build, routed
 from test_routed import HALF, TYPES, make_routing, near, plain_choice, wide
 
 gpu = pytest.mark.gpu
@@ -167,3 +168,69 @@ def test_operators_inside_a_function():
     assert torch.allclose(y.detach().double().cpu(), expected.detach(), rtol=2 * 2.0 ** -8, atol=2.0)
     assert torch.allclose(x.grad.double().cpu(), xd.grad, rtol=2 * 2.0 ** -8, atol=0.5)
     assert torch.allclose(w.grad.double().cpu(), wd.grad, rtol=2.0 ** -8, atol=0.5)
+
+
+SHARED_LIMIT = r"""
+// AllowShared with the runtime's calls replaced: the limit that a kernel has, as two threads raise it.
+#include <cuda_runtime.h>
+
+#include <chrono>
+#include <condition_variable>
+#include <mutex>
+#include <thread>
+
+std::mutex g_mutex;
+std::condition_variable g_changed;
+int g_limit = 0;
+bool g_shrunk = false, g_large_set = false, g_small_done = false;
+
+cudaError_t FakeDevice(int* device) { return *device = 0, cudaSuccess; }
+
+template <typename Kernel>
+cudaError_t FakeAttribute(Kernel*, cudaFuncAttribute, int bytes) {
+  std::unique_lock<std::mutex> lock(g_mutex);
+  g_shrunk = g_shrunk || bytes < g_limit;
+  g_limit = bytes;
+  if (bytes == 200000) {   // the other thread's call comes before this one returns, if it can
+    g_large_set = true;
+    g_changed.notify_all();
+    g_changed.wait_for(lock, std::chrono::milliseconds(500), [] { return g_small_done; });
+  }
+  return cudaSuccess;
+}
+#define cudaGetDevice FakeDevice
+#define cudaFuncSetAttribute FakeAttribute
+#include "routed.cuh"
+
+namespace t0b {
+void Check(cudaError_t, const char*) {}
+}
+
+__global__ void Nothing() {}
+
+int main() {
+  std::thread large([] { t0b::AllowShared<Nothing>(200000); });
+  std::thread small([] {
+    {
+      std::unique_lock<std::mutex> lock(g_mutex);
+      g_changed.wait(lock, [] { return g_large_set; });
+    }
+    t0b::AllowShared<Nothing>(60000);
+    const std::lock_guard<std::mutex> lock(g_mutex);
+    g_small_done = true;
+    g_changed.notify_all();
+  });
+  large.join();
+  small.join();
+  t0b::AllowShared<Nothing>(200000);
+  return g_shrunk || g_limit != 200000;
+}
+"""
+
+
+def test_a_kernels_shared_memory_limit_only_grows(tmp_path):
+    source, program = tmp_path / "limit.cu", tmp_path / "limit"
+    source.write_text(SHARED_LIMIT)
+    subprocess.run([build.nvcc(), *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr", "-I", str(build.CSRC), str(source),
+                    "-o", str(program)], check=True)
+    assert subprocess.run([str(program)], timeout=60).returncode == 0
