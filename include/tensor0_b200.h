@@ -282,10 +282,11 @@ int t0b_sector_gemm(int32_t dtype, int64_t sectors, const int64_t* host_table,
  * per token at run time, on the device, with their gradients.  An entry is one
  * (token, slot) pair, number token * top_k + slot; expert-ordered row p holds
  * entry rows[p], and expert e's rows are [offsets[e], offsets[e + 1]).  Entries
- * without an expert are ordered last, from offsets[experts] on.  Row strides are
- * in elements.  rows, positions and offsets are the device arrays t0b_route
- * writes; kernels skip an address outside the stated operand.  Outputs are
- * contiguous and must not overlap inputs.
+ * without an expert are ordered last, from offsets[experts] on.  There are at
+ * most 2^31 - 256 entries (tokens * top_k).  Row strides are in elements.  rows,
+ * positions and offsets are the device arrays t0b_route writes; kernels skip an
+ * address outside the stated operand.  Outputs are contiguous and must not
+ * overlap inputs.
  *
  * t0b_route: scores s = softmax (score 0) or sigmoid (score 1) of the token's
  * logits (F32, F16, BF16); choice c = s + bias, or the logits where bias is
@@ -297,8 +298,8 @@ int t0b_sector_gemm(int32_t dtype, int64_t sectors, const int64_t* host_table,
  * softmax a NaN or +inf logit makes the token's weights NaN; its choice goes by
  * the scores without the NaN logits, and by their limits at +inf.  Missing
  * choices have index -1, weight 0 and position -1.  experts <= 512, top_k <= 32,
- * groups <= 32, tokens * top_k < 2^31.  workspace: t0b_route_workspace() bytes,
- * 4-byte aligned (may be NULL when that is 0).
+ * groups <= 32.  workspace: t0b_route_workspace() bytes, 4-byte aligned (may be
+ * NULL when that is 0).
  */
 size_t t0b_route_workspace(int64_t tokens, int32_t experts);
 int t0b_route(int32_t dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups,

@@ -15,7 +15,10 @@ using t0b::Disjoint;
 using t0b::Guard;
 using t0b::InvalidArgument;
 
-constexpr int64_t kMaxEntries = (int64_t{1} << 31) - 1;
+constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1;         // gated rows, row strides
+// Router and products index entries in 32 bits, up to a tile of rows or a
+// block's tokens past the last one.
+constexpr int64_t kMaxEntries = (int64_t{1} << 31) - 256;
 constexpr int32_t kMaxWidth = 1 << 23;   // blocks of 256 columns fit a grid axis
 
 uint64_t Half(int32_t dtype, const char* what) {
@@ -32,7 +35,7 @@ void Require(bool condition, const char* message) {
 uint64_t Operand(const void* data, int64_t rows, int64_t width, int64_t stride, uint64_t item, const char* what) {
   if (rows < 0 || width < 0) throw InvalidArgument(std::string(what) + " sizes must be nonnegative");
   if (stride < width) throw InvalidArgument(std::string(what) + " row stride is below the row's width");
-  if (stride > kMaxEntries) throw InvalidArgument(std::string(what) + " row stride must be at most 2^31 - 1");
+  if (stride > kMaxRows) throw InvalidArgument(std::string(what) + " row stride must be at most 2^31 - 1");
   if (rows == 0 || width == 0) return 0;
   if (data == nullptr) throw InvalidArgument(std::string(what) + " buffer is null");
   if (reinterpret_cast<uintptr_t>(data) % item != 0) {
@@ -66,7 +69,7 @@ void Separate(std::initializer_list<Extent> outputs, std::initializer_list<Exten
 }
 
 void RequireRouting(int64_t entries, int32_t experts, int32_t top_k) {
-  Require(entries >= 0 && entries <= kMaxEntries, "routed entries must be at most 2^31 - 1");
+  Require(entries >= 0 && entries <= kMaxEntries, "routed entries must be at most 2^31 - 256");
   Require(experts >= 1 && experts <= t0b::kRouteMaxExperts, "routed operators take 1 to 512 experts");
   Require(top_k >= 1 && top_k <= t0b::kRouteMaxTopK, "top_k must be from 1 to 32");
   Require(entries % top_k == 0, "routed entries must be a multiple of top_k");
@@ -79,7 +82,7 @@ uint64_t RequireScore(int32_t dtype, int64_t tokens, int32_t experts, int32_t to
   Require(experts >= 1 && experts <= t0b::kRouteMaxExperts, "routed operators take 1 to 512 experts");
   Require(top_k >= 1 && top_k <= t0b::kRouteMaxTopK && top_k <= experts,
           "top_k must be from 1 to 32 and at most the number of experts");
-  Require(tokens <= kMaxEntries / top_k, "routed entries must be at most 2^31 - 1");
+  Require(tokens <= kMaxEntries / top_k, "routed entries must be at most 2^31 - 256");
   Require(score == 0 || score == 1, "router score must be 0 (softmax) or 1 (sigmoid)");
   Require(renormalize == 0 || renormalize == 1, "renormalize must be zero or one");
   Require(std::isfinite(scale), "router scale must be finite");
@@ -94,7 +97,7 @@ void RequireGroup(int32_t width, int32_t group) {
 // The routing of gated rows: all given or none.
 uint64_t RequireRowWeights(const float* weights, const int32_t* row_entries, const int32_t* offsets, int32_t experts,
                            int64_t rows) {
-  Require(rows >= 0 && rows <= kMaxEntries, "gated rows must be at most 2^31 - 1");
+  Require(rows >= 0 && rows <= kMaxRows, "gated rows must be at most 2^31 - 1");
   const bool some = weights != nullptr || row_entries != nullptr || offsets != nullptr;
   if (!some) return 0;
   Require((weights != nullptr && row_entries != nullptr && offsets != nullptr) || rows == 0,
@@ -280,7 +283,7 @@ int t0b_routed_sum(int32_t dtype, int64_t tokens, int32_t top_k, int32_t width, 
     const uint64_t item = Half(dtype, "routed sums");
     Require(tokens >= 0, "token count must be nonnegative");
     Require(top_k >= 1 && top_k <= t0b::kRouteMaxTopK, "top_k must be from 1 to 32");
-    Require(tokens <= kMaxEntries / top_k, "routed entries must be at most 2^31 - 1");
+    Require(tokens <= kMaxEntries / top_k, "routed entries must be at most 2^31 - 256");
     Require(width >= 1 && width <= kMaxWidth, "sum width must be from 1 to 2^23");
     const int64_t entries = tokens * top_k;
     const uint64_t y_bytes = Operand(y, entries, width, y_stride, item, "sum");
@@ -379,7 +382,7 @@ int t0b_checkpoint_load(int32_t dtype, int64_t row_count, int32_t width, int32_t
   return Guard(error, error_size, [&] {
     Require(dtype == T0B_F32 || dtype == T0B_F16 || dtype == T0B_BF16, "checkpoints load as F32, F16 or BF16");
     RequireGroup(width, group);
-    Require(row_count >= 0 && row_count <= kMaxEntries, "gated rows must be at most 2^31 - 1");
+    Require(row_count >= 0 && row_count <= kMaxRows, "gated rows must be at most 2^31 - 1");
     const int64_t groups = (int64_t{width} + group - 1) / group;
     const uint64_t code_bytes = Packed(codes, row_count, int64_t{2} * width, 1, "checkpoint code");
     const uint64_t scale_bytes = Packed(scales, row_count, 2 * groups, 4, "checkpoint scale");

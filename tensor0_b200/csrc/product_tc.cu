@@ -559,14 +559,15 @@ void ByWidth(const ProductArgs& p, bool bf16, cudaStream_t stream) {
 
 }  // namespace
 
-// Every operand row starts on a 16-byte boundary and no tile index passes 32 bits.
+// Every operand row starts on a 16-byte boundary and no tile index passes 32 bits,
+// nor does one that is a turn of the blocks further.
 bool TensorCoreProduct(int kind, const ProductArgs& p) {
   const auto aligned = [](const void* data) { return reinterpret_cast<uintptr_t>(data) % 16 == 0; };
   const int64_t width = kind == kProductTransposed ? p.inner : p.outer;
   const int64_t rows = kind == kProductWeightGrad ? int64_t{p.experts} * (p.inner + kTileRows) : p.entries + int64_t{p.experts} * kTileRows;
   return p.entries > 0 && p.inner % 8 == 0 && p.outer % 8 == 0 && p.x_stride % 8 == 0 &&
          (kind != kProductWeightGrad || p.w_stride % 8 == 0) && aligned(p.x) && aligned(p.w) && aligned(p.out) &&
-         rows / kTileRows * ((width + 63) / 64) < (int64_t{1} << 31);
+         rows / kTileRows * ((width + 63) / 64) < (int64_t{1} << 31) - 4096;
 }
 
 void LaunchTensorCoreProduct(int kind, int32_t dtype, const ProductArgs& args, cudaStream_t stream) {

@@ -262,7 +262,7 @@ __device__ __forceinline__ int PickPacked(const uint32_t (&key)[V], int top_k, b
 template <typename T, int V, bool kByLogit>
 __device__ __forceinline__ void SelectTokens(const RouteArgs& a, int64_t begin, int64_t end, float* values, bool vector) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  // tokens * top_k and a row stride are below 2^31: 32-bit indices, which cost a
+  // A row stride is below 2^31, and tokens * top_k by 256: 32-bit indices, which cost a
   // tenth of the instructions less than 64-bit ones.
   const int stride = static_cast<int>(a.logit_stride), last = static_cast<int>(end);
   const bool bias_vector = reinterpret_cast<uintptr_t>(a.bias) % (V * 4 < 16 ? V * 4 : 16) == 0;
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs
   LetNextStart();
   WaitForPrevious();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t = static_cast<int>(blockIdx.x) * (kRouteThreads / 32) + warp;   // tokens * top_k is below 2^31
+  const int t = static_cast<int>(blockIdx.x) * (kRouteThreads / 32) + warp;   // there are at most 2^31 - 256 tokens
   if (t >= static_cast<int>(a.tokens)) return;
   const T* row = static_cast<const T*>(a.logits) + int64_t{t} * static_cast<int>(a.logit_stride);
   int mine = -1;

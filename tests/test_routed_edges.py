@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from tensor0_b200 import build, routed
-from test_routed import HALF, TYPES, make_routing, near, plain_choice, wide
+from test_routed import A, B, C, D, E, F, HALF, TYPES, call, make_routing, near, plain_choice, wide
 
 gpu = pytest.mark.gpu
 
@@ -234,3 +234,24 @@ def test_a_kernels_shared_memory_limit_only_grows(tmp_path):
     subprocess.run([build.nvcc(), *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr", "-I", str(build.CSRC), str(source),
                     "-o", str(program)], check=True)
     assert subprocess.run([str(program)], timeout=60).returncode == 0
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Refusals
+
+MOST = (1 << 31) - 256          # entries
+
+
+@pytest.mark.parametrize("entries", [MOST + 1, (1 << 31) - 1])
+def test_more_entries_than_the_indices_hold_are_refused(entries):
+    """Kernels form indices of up to a tile past the last entry in 32 bits.  (The missing operand is refused later.)"""
+    for name, arguments in [
+            ("t0b_route", (11, entries, 8, 1, 1, 1, 1, 0, 1, 1.0, None, 8, None, None, A, B, C, D, E, F, 1 << 40)),
+            ("t0b_route_backward", (11, entries, 8, 1, 0, 1, 1.0, None, 8, B, C, D)),
+            ("t0b_routed_product", (10, 0, entries, 2, 1, 16, 32, 0, None, entries, 16, B, C, D, E)),
+            ("t0b_routed_product", (10, 1, entries, 2, 1, 16, 32, 1, None, entries, 32, B, C, D, E)),
+            ("t0b_routed_weight_grad", (10, entries, 2, 1, 16, 32, 0, None, entries, 16, 0, B, entries, 32, C, D, E)),
+            ("t0b_routed_sum", (10, entries, 1, 8, None, 8, B, C)),
+            ("t0b_routed_matvec4", (10, entries, 2, 1, 64, 32, 32, 1, None, entries, 64, B, C, D, E, F))]:
+        status, text = call(name, *arguments)
+        assert status == 1 and "2^31 - 256" in text, (name, text)
