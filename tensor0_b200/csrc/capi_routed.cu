@@ -94,19 +94,25 @@ void RequireGroup(int32_t width, int32_t group) {
   Require(group == 32 || group == 64 || group == 128, "checkpoint group must be 32, 64 or 128");
 }
 
+// Bytes of a gated routing's arrays: its weights and its rows each, and its offsets.
+struct RowWeightBytes {
+  uint64_t entries = 0, offsets = 0;
+};
+
 // The routing of gated rows: all given or none.
-uint64_t RequireRowWeights(const float* weights, const int32_t* row_entries, const int32_t* offsets, int32_t experts,
-                           int64_t rows) {
+RowWeightBytes RequireRowWeights(const float* weights, const int32_t* row_entries, const int32_t* offsets,
+                                 int32_t experts, int64_t rows) {
   Require(rows >= 0 && rows <= kMaxRows, "gated rows must be at most 2^31 - 1");
   const bool some = weights != nullptr || row_entries != nullptr || offsets != nullptr;
-  if (!some) return 0;
+  if (!some) return {};
   Require((weights != nullptr && row_entries != nullptr && offsets != nullptr) || rows == 0,
           "a gated routing is its weights, its rows and its offsets");
   Require(experts >= 1 && experts <= t0b::kRouteMaxExperts, "routed operators take 1 to 512 experts");
-  Packed(weights, rows, 1, 4, "weight");
+  RowWeightBytes bytes;
+  bytes.entries = Packed(weights, rows, 1, 4, "weight");
   Packed(row_entries, rows, 1, 4, "row");
-  if (rows != 0) Packed(offsets, experts + 1, 1, 4, "offset");
-  return static_cast<uint64_t>(rows) * 4;
+  if (rows != 0) bytes.offsets = Packed(offsets, experts + 1, 1, 4, "offset");
+  return bytes;
 }
 
 void Product(int kind, int32_t dtype, const t0b::ProductArgs& a, uint64_t out_width, int64_t out_rows, void* stream) {
@@ -311,7 +317,7 @@ int t0b_gated_save(int32_t dtype, int64_t row_count, int32_t width, int32_t grou
   return Guard(error, error_size, [&] {
     const uint64_t item = Half(dtype, "gated activations");
     RequireGroup(width, group);
-    const uint64_t entry_bytes = RequireRowWeights(weights, row_entries, offsets, experts, row_count);
+    const RowWeightBytes routing = RequireRowWeights(weights, row_entries, offsets, experts, row_count);
     const int64_t groups = (int64_t{width} + group - 1) / group;
     const uint64_t h_bytes = Operand(h, row_count, int64_t{2} * width, h_stride, item, "activation input");
     const uint64_t a_bytes = Packed(a, row_count, width, item, "activation");
@@ -320,7 +326,7 @@ int t0b_gated_save(int32_t dtype, int64_t row_count, int32_t width, int32_t grou
     const uint64_t code_bytes = Packed(codes, kept, int64_t{2} * width, 1, "checkpoint code");
     const uint64_t scale_bytes = Packed(scales, kept, 2 * groups, 4, "checkpoint scale");
     Separate({{a, a_bytes}, {codes, code_bytes}, {scales, scale_bytes}},
-             {{h, h_bytes}, {weights, entry_bytes}, {row_entries, entry_bytes}});
+             {{h, h_bytes}, {weights, routing.entries}, {row_entries, routing.entries}, {offsets, routing.offsets}});
     if (row_count == 0) return;
     t0b::GatedArgs args{};
     args.h = h;
@@ -346,7 +352,7 @@ int t0b_gated_backward(int32_t dtype, int64_t row_count, int32_t width, int32_t 
   return Guard(error, error_size, [&] {
     const uint64_t item = Half(dtype, "gated activations");
     RequireGroup(width, group);
-    const uint64_t entry_bytes = RequireRowWeights(weights, row_entries, offsets, experts, row_count);
+    const RowWeightBytes routing = RequireRowWeights(weights, row_entries, offsets, experts, row_count);
     const int64_t groups = (int64_t{width} + group - 1) / group;
     const uint64_t code_bytes = Packed(codes, row_count, int64_t{2} * width, 1, "checkpoint code");
     const uint64_t scale_bytes = Packed(scales, row_count, 2 * groups, 4, "checkpoint scale");
@@ -355,8 +361,8 @@ int t0b_gated_backward(int32_t dtype, int64_t row_count, int32_t width, int32_t 
     const uint64_t h_bytes = Packed(h_grad, row_count, int64_t{2} * width, item, "input gradient");
     const uint64_t w_bytes = weights_grad != nullptr ? Packed(weights_grad, row_count, 1, 4, "weight gradient") : 0;
     Separate({{a, a_bytes}, {h_grad, h_bytes}, {weights_grad, w_bytes}},
-             {{codes, code_bytes}, {scales, scale_bytes}, {a_grad, grad_bytes}, {weights, entry_bytes},
-              {row_entries, entry_bytes}});
+             {{codes, code_bytes}, {scales, scale_bytes}, {a_grad, grad_bytes}, {weights, routing.entries},
+              {row_entries, routing.entries}, {offsets, routing.offsets}});
     if (row_count == 0) return;
     t0b::GatedArgs args{};
     args.codes = const_cast<int8_t*>(codes);

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from tensor0_b200 import build, routed
-from test_routed import A, B, C, D, E, F, HALF, TYPES, call, make_routing, near, plain_choice, wide
+from test_routed import A, B, C, D, E, F, G, H, HALF, TYPES, call, make_routing, near, plain_choice, wide
 
 gpu = pytest.mark.gpu
 
@@ -255,3 +255,17 @@ def test_more_entries_than_the_indices_hold_are_refused(entries):
             ("t0b_routed_matvec4", (10, entries, 2, 1, 64, 32, 32, 1, None, entries, 64, B, C, D, E, F))]:
         status, text = call(name, *arguments)
         assert status == 1 and "2^31 - 256" in text, (name, text)
+
+
+@pytest.mark.parametrize("name, arguments", [
+    ("t0b_gated_save", (10, 4, 8, 32, A, 16, B, C, D, 2, D, E, F)),                     # a
+    ("t0b_gated_save", (10, 4, 8, 32, A, 16, B, C, D + 8, 2, E, D, F)),                 # codes, from 8 bytes before on
+    ("t0b_gated_save", (10, 4, 8, 32, A, 16, B, C, D, 2, E, F, D)),                     # scales
+    ("t0b_gated_backward", (10, 4, 8, 32, A, B, C, 8, E, F, D, 2, D, G, H)),            # h_grad
+    ("t0b_gated_backward", (10, 4, 8, 32, A, B, C, 8, E, F, D, 2, G, D, H)),            # a
+    ("t0b_gated_backward", (10, 4, 8, 32, A, B, C, 8, E, F, D, 2, G, H, D)),            # weights_grad
+])
+def test_gated_results_over_the_routings_offsets_are_refused(name, arguments):
+    """Every block reads the offsets while others write."""
+    status, text = call(name, *arguments)
+    assert status == 1 and "overlap" in text, text
