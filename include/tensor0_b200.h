@@ -298,8 +298,8 @@ int t0b_sector_gemm(int32_t dtype, int64_t sectors, const int64_t* host_table,
  * softmax a NaN or +inf logit makes the token's weights NaN; its choice goes by
  * the scores without the NaN logits, and by their limits at +inf.  Missing
  * choices have index -1, weight 0 and position -1.  experts <= 512, top_k <= 32,
- * groups <= 32.  workspace: t0b_route_workspace() bytes, 4-byte aligned (may be
- * NULL when that is 0).
+ * groups <= 32.  workspace: t0b_route_workspace() bytes for the current device,
+ * 4-byte aligned (may be NULL when that is 0, as it is for refused sizes).
  */
 size_t t0b_route_workspace(int64_t tokens, int32_t experts);
 int t0b_route(int32_t dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups,

@@ -102,6 +102,11 @@ class Place {
     if (!tensor.is_cuda()) throw Refusal("routed storage must be a CUDA tensor (there is no CPU fallback)");
     if (tensor.get_device() != index_) throw Refusal("routed operands must be on one device");
   }
+  // Bytes of workspace that a route needs on the device.
+  size_t RouteWorkspace(int64_t tokens, int32_t experts) const {
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(index_));
+    return t0b_route_workspace(tokens, experts);
+  }
   // Runs `entry(stream, error, error size)` on the device's current stream.
   template <typename Entry>
   void Run(Entry&& entry) const {
@@ -271,7 +276,7 @@ PyObject* Route(PyObject*, Arguments args, Py_ssize_t count) {
     const Routing out(place, args[10]);
     const int32_t* chosen = Packed<int32_t>(place, *out.chosen, {tokens, top_k}, at::kInt, "routing experts");
     const int32_t* offsets = Packed<int32_t>(place, *out.offsets_tensor, {experts + 1}, at::kInt, "routing offsets");
-    const size_t size = t0b_route_workspace(tokens, experts);
+    const size_t size = place.RouteWorkspace(tokens, experts);
     Tensor workspace;
     if (size != 0) workspace = at::empty({static_cast<int64_t>(size)}, logits.options().dtype(at::kByte));
     void* work = size != 0 ? workspace.data_ptr() : nullptr;

@@ -147,7 +147,8 @@ void Product(int kind, int32_t dtype, const t0b::ProductArgs& a, uint64_t out_wi
 extern "C" {
 
 size_t t0b_route_workspace(int64_t tokens, int32_t experts) {
-  return tokens < 0 || experts < 1 ? 0 : t0b::RouteWorkspace(tokens, experts);
+  if (tokens < 0 || tokens > kMaxEntries || experts < 1 || experts > t0b::kRouteMaxExperts) return 0;
+  return t0b::RouteWorkspace(tokens, experts);
 }
 
 int t0b_route(int32_t dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups,

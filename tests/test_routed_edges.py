@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from tensor0_b200 import build, routed
+from tensor0_b200 import _native, build, routed
 from test_routed import A, B, C, D, E, F, G, H, HALF, TYPES, call, make_routing, near, plain_choice, wide
 
 gpu = pytest.mark.gpu
@@ -269,3 +269,11 @@ def test_gated_results_over_the_routings_offsets_are_refused(name, arguments):
     """Every block reads the offsets while others write."""
     status, text = call(name, *arguments)
     assert status == 1 and "overlap" in text, text
+
+
+@pytest.mark.parametrize("tokens, experts", [(1000, 513), (1000, 1 << 30), (MOST + 1, 8), (1 << 60, 8), (-1, 8), (1000, 0)])
+def test_a_route_that_is_refused_needs_no_workspace(tokens, experts):
+    """The binding asks for the size before the router checks its arguments: no memory for what it refuses."""
+    build.build()
+    assert _native.lib().t0b_route_workspace(tokens, experts) == 0
+    assert _native.lib().t0b_route_workspace(1000, 512) > 0
