@@ -10,6 +10,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -101,6 +102,11 @@ class Place {
   void Holds(const Tensor& tensor) const {
     if (!tensor.is_cuda()) throw Refusal("routed storage must be a CUDA tensor (there is no CPU fallback)");
     if (tensor.get_device() != index_) throw Refusal("routed operands must be on one device");
+    // Recorded calls would leave this operator out of the gradient without a word.
+    if (tensor.requires_grad() && c10::GradMode::is_enabled()) {
+      throw Refusal("an operand requires a gradient, which routed operators do not record: call them and their backward "
+                    "operators in a torch.autograd.Function, or under torch.no_grad()");
+    }
   }
   // Bytes of workspace that a route needs on the device.
   size_t RouteWorkspace(int64_t tokens, int32_t experts) const {
@@ -270,7 +276,10 @@ PyObject* Route(PyObject*, Arguments args, Py_ssize_t count) {
     const int32_t best = Small(args[4], "group_best"), renormalize = Flag(args[6]);
     const float scale = Real(args[7]);
     const float* bias = nullptr;
-    if (args[8] != Py_None) bias = Packed<float>(place, Get(args[8], "bias"), {experts}, at::kFloat, "bias");
+    if (args[8] != Py_None) {
+      const Tensor& given = Get(args[8], "bias");   // has no gradient: it enters the choice only
+      bias = Packed<float>(place, given.requires_grad() ? given.detach() : given, {experts}, at::kFloat, "bias");
+    }
     const uint8_t* mask = nullptr;
     if (args[9] != Py_None) mask = Packed<uint8_t>(place, Get(args[9], "mask"), {tokens}, at::kBool, "mask");
     const Routing out(place, args[10]);

@@ -16,8 +16,12 @@ tokens, excluded experts) come last; their rows are zeros.
 
 As for the stride engine, storage is CUDA tensors, calls are ordered on the
 current stream of the storage's device, nothing synchronizes, and there is no
-CPU fallback.  ``out`` takes preallocated results, so that a captured or
-latency-bound step allocates nothing.
+CPU fallback.  ``out`` takes preallocated results; what is not given comes
+from torch's allocator, as the workspace of a route of more than 64 tokens does.
+
+The operators record nothing for autograd: an operand that requires a gradient
+is refused while gradients are recorded.  A ``torch.autograd.Function`` around
+them calls the backward operators in its own backward pass.
 """
 
 from __future__ import annotations
@@ -184,6 +188,7 @@ def checkpoint_load(checkpoint: Checkpoint, dtype: torch.dtype = torch.float32) 
     return _routed.checkpoint_load(checkpoint, _FLOAT[dtype])
 
 
+@torch.no_grad()
 def pack_int4(w: torch.Tensor, group: int = 128) -> Int4Weights:
     """``w`` [experts, inner, outer] in 4 bits: per group of ``group`` inner neighbours the scale max|w| / 7 (in w's
     type) and whole numbers from -7 to 7.  Done once per model, in plain torch."""

@@ -136,6 +136,61 @@ def test_a_threads_first_call(name):
     assert torch.equal(found[0], expected)
 
 
+# ----------------------------------------------------------------------------------------------------------------
+# Autograd
+
+
+@gpu
+def test_autograd_is_refused_and_not_ignored():
+    _, r = make_routing(6, 4, 2, 1)
+    x, w = torch.randn(6, 32).half().cuda(), torch.randn(4, 32, 16).half().cuda()
+    h, logits = torch.randn(12, 32).half().cuda(), torch.randn(6, 4).cuda()
+    a, kept = routed.gated_save(h)
+    four = routed.pack_int4(w, 32)
+    calls = [
+        (lambda t: routed.route(t, 2), logits),
+        (lambda t: routed.route_backward(t, r, torch.ones(6, 2).cuda()), logits),
+        (lambda t: routed.route_backward(logits, r, t), torch.ones(6, 2).cuda()),
+        (lambda t: routed.routed_matmul(t, w, r, gather=True), x),
+        (lambda t: routed.routed_matmul(x, t, r, gather=True), w),
+        (lambda t: routed.routed_matmul(x, w, r, gather=True, out=t), torch.empty(12, 16).half().cuda()),
+        (lambda t: routed.routed_weight_grad(t, h, r, gather_x=True), x),
+        (lambda t: routed.routed_weight_grad(x, t, r, gather_x=True), h),
+        (lambda t: routed.routed_sum(t, r), h),
+        (lambda t: routed.gated_save(t), h),
+        (lambda t: routed.gated(t), h),
+        (lambda t: routed.gated_save(h, routing=r._replace(weights=t)), r.weights.clone()),
+        (lambda t: routed.gated_backward(kept, t), a.clone()),
+        (lambda t: routed.checkpoint_load(kept._replace(scales=t)), kept.scales.clone()),
+        (lambda t: routed.routed_matvec(t, four, r, gather=True), x),
+        (lambda t: routed.routed_matvec(x, four._replace(scales=t), r, gather=True), four.scales.clone()),
+    ]
+    for number, (call, tensor) in enumerate(calls):
+        leaf = tensor.detach().clone().requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            call(leaf)
+            raise AssertionError(f"call {number} was taken")
+        with torch.no_grad():
+            call(leaf)
+        call(leaf.detach())
+
+
+@gpu
+def test_weights_that_train_are_packed_without_a_graph():
+    w = torch.randn(2, 64, 8).bfloat16().cuda().requires_grad_()
+    packed = routed.pack_int4(w, 32)
+    assert not packed.scales.requires_grad
+    plain = routed.pack_int4(w.detach(), 32)
+    assert torch.equal(packed.codes, plain.codes) and torch.equal(packed.scales, plain.scales)
+
+
+@gpu
+def test_a_bias_has_no_gradient_and_is_taken():
+    logits, bias = torch.randn(9, 8).cuda(), torch.randn(8).cuda()
+    r = routed.route(logits, 2, bias=bias.clone().requires_grad_())
+    assert all(torch.equal(a, b) for a, b in zip(r, routed.route(logits, 2, bias=bias)))
+
+
 class Product(torch.autograd.Function):
     """How a user joins the operators to autograd: each backward operator in its own Function."""
     @staticmethod
