@@ -313,6 +313,9 @@ PyObject* RouteBackward(PyObject*, Arguments args, Py_ssize_t count) {
     const int32_t code = FloatCode(logits.scalar_type(), "logits"), score = Score(args[3]);
     const Rows rows = Matrix(place, logits, tokens, experts, "logits");
     const Routing r(place, args[1]);
+    if (r.experts != experts) {
+      throw Refusal("the routing has " + std::to_string(r.experts) + " experts, the logits " + std::to_string(experts));
+    }
     const int32_t* chosen = Packed<int32_t>(place, *r.chosen, {tokens, r.top_k}, at::kInt, "routing experts");
     const float* grad = Packed<float>(place, Get(args[2], "weights_grad"), {tokens, r.top_k}, at::kFloat, "weights_grad");
     const int32_t renormalize = Flag(args[4]);

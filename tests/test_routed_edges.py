@@ -332,3 +332,12 @@ def test_a_route_that_is_refused_needs_no_workspace(tokens, experts):
     build.build()
     assert _native.lib().t0b_route_workspace(tokens, experts) == 0
     assert _native.lib().t0b_route_workspace(1000, 512) > 0
+
+
+@gpu
+@pytest.mark.parametrize("experts", [4, 16])
+def test_router_gradient_refuses_another_routers_routing(experts):
+    logits = torch.randn(10, 8).cuda()
+    r = routed.route(torch.randn(10, experts).cuda(), 2)
+    with pytest.raises(ValueError, match="experts"):
+        routed.route_backward(logits, r, torch.ones(10, 2).cuda())
