@@ -12,6 +12,10 @@
 // Both are exact.  What is added to each weight (8 too much, or 24) is taken
 // off by starting a group's 32-bit sum at minus that times the sum of x, and
 // the scale multiplies the group's sum, so nothing is rounded before the result.
+// Values that these sums do not hold, infinities or BF16 ones from 2^115 on, are
+// rare: eight token rows with one among them are computed again, by the formula as
+// it stands (MvAgain; 16 tokens to 4 of 64 experts at 4096 x 2048 with an infinity
+// each 1.4 ms).  Looking for them costs 0.2 us of a small call, 1 % of a large one.
 //
 // Two blocks per streaming multiprocessor walk tasks: some weight rows of one
 // expert and eight of its token rows.  Eight warps compute: 16-row tiles times
@@ -113,6 +117,16 @@ struct MvSum {
 template <typename T> constexpr float kMvExcess = std::is_same<T, __half>::value ? -8.0f * 0x1p-24f : -24.0f;
 template <typename T> constexpr float kMvSize = std::is_same<T, __half>::value ? 0x1p24f : 1.0f;
 
+// Added to a 16-bit magnitude it sets the top bit of one that is too large for the
+// sums: an infinity or NaN, and of BF16 what 128 weights of up to 31 could take
+// past 2^127.  (F16 values that are finite stay far below.)
+template <typename T> constexpr uint32_t kMvAbove = std::is_same<T, __half>::value ? 0x0400u : 0x0700u;
+template <typename T> __device__ __forceinline__ uint32_t MvAbove(const uint4& q) {
+  constexpr uint32_t kMagnitudes = 0x7fff7fffu, kAdd = kMvAbove<T> * 0x10001u;
+  return (((q.x & kMagnitudes) + kAdd) | ((q.y & kMagnitudes) + kAdd) | ((q.z & kMagnitudes) + kAdd) |
+          ((q.w & kMagnitudes) + kAdd)) & 0x80008000u;
+}
+
 // Groups of 32: lanes t and t ^ 2 swap a word, so that each of a half's two
 // groups is spread over the four lanes and a matrix instruction stays in one.
 __device__ __forceinline__ void Swap(uint2& w, int t) {
@@ -122,8 +136,9 @@ __device__ __forceinline__ void Swap(uint2& w, int t) {
 }
 
 struct MvShared {
-  uint64_t full[kMvStages], empty[kMvStages], laid[2], used[2];
+  uint64_t full[kMvStages], empty[kMvStages], laid[2], used[2], seen, stored;
   volatile int failed;
+  volatile int above;                // x has values too large for the sums
   int present;                       // experts that have rows
   int experts[kRouteMaxExperts];     // and which
   float sums[kMvWarps][16][9];
@@ -134,6 +149,50 @@ struct MvTask {
   int64_t first, begin, end;   // first: the expert's first weight row
   int row0;
 };
+
+// One of four warps: its share of a task's weight rows times eight token rows, if
+// one of these has a value that is too large for the sums, by the formula as it
+// stands and straight from memory.  Lanes take every 32nd eight of the deep values.
+template <typename T, int kGroup, int kRows>
+__device__ __forceinline__ void MvAgain(const MatvecArgs& a, const MvTask& task, int64_t p0, int warp) {
+  const int lane = threadIdx.x & 31, groups = a.inner / kGroup, rows = static_cast<int>(min(int64_t{8}, task.end - p0));
+  const uint16_t* mine = nullptr;   // lane n: token row n, null if there is none
+  if (lane < rows) {
+    const int64_t token = a.gather != 0 ? a.rows[p0 + lane] / a.top_k : p0 + lane;
+    if (token >= 0 && token < a.x_rows) mine = static_cast<const uint16_t*>(a.x) + token * a.x_stride;
+  }
+  uint32_t above = 0;
+#pragma unroll 1
+  for (int n = 0; n < rows; ++n) {
+    const uint16_t* x = reinterpret_cast<const uint16_t*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(mine), n));
+    if (x == nullptr) continue;
+#pragma unroll 1
+    for (int k = lane; k < a.inner; k += 32) above |= ((x[k] & 0x7fffu) + kMvAbove<T>) & 0x8000u;
+  }
+  if (!__any_sync(kFull, above != 0u)) return;
+#pragma unroll 1
+  for (int row = task.row0 + warp; row < min(task.row0 + kRows, a.outer); row += kMvLayout / 32) {
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.codes + (task.first + row) * (a.inner / 2));
+    const T* scales = static_cast<const T*>(a.scales) + (task.first + row) * groups;
+#pragma unroll 1
+    for (int n = 0; n < rows; ++n) {
+      const uint16_t* x = reinterpret_cast<const uint16_t*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(mine), n));
+      float sum = 0.0f;
+#pragma unroll 1
+      for (int u = lane; u < a.inner / 8 && x != nullptr; u += 32) {
+        const uint32_t word = codes[u];
+        const float scale = ToFloat(scales[u / (kGroup / 8)]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {   // weights are exact in 32 bits
+          sum = fmaf(static_cast<float>(static_cast<int>((word >> (4 * i)) & 15u) - 8) * scale, Unpack2<T>(x[u * 8 + i]).x, sum);
+        }
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+      if (lane == 0) static_cast<T*>(a.out)[(p0 + n) * a.outer + row] = FromFloat<T>(sum);
+    }
+  }
+}
 
 template <typename T, int kGroup, int kParts>
 __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
@@ -162,6 +221,9 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
       BarrierInit(SharedAddress(&s.used[i]), kMvWarps);
     }
     s.failed = 0;
+    BarrierInit(SharedAddress(&s.seen), kMvLayout / 32);
+    BarrierInit(SharedAddress(&s.stored), kMvWarps);
+    s.above = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (tid == 32) PrefetchMap(&map);
@@ -232,7 +294,7 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
         out[i] = FromFloat<T>(0.0f);
       }
     }
-    uint32_t turn = 0;
+    uint32_t turn = 0, above = 0;
     for (int index = blockIdx.x; index < tasks; index += gridDim.x) {
       const MvTask task = task_at(index);
       const uint16_t* source = static_cast<const uint16_t*>(a.scales) + (task.first + task.row0) * groups;
@@ -319,6 +381,7 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
               for (int i = 0; i < kUnits; ++i) {
                 const int u = i * kMvLayout + lt;
                 const uint4 q = v[n][i];
+                above |= MvAbove<T>(q);
                 const float2 f0 = Unpack2<T>(q.x), f1 = Unpack2<T>(q.y), f2 = Unpack2<T>(q.z), f3 = Unpack2<T>(q.w);
                 float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
 #pragma unroll
@@ -347,6 +410,19 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
           BarrierArrive(SharedAddress(&s.laid[buffer]));
         }
       }
+    }
+    // Token rows with values too large for the sums: again, over what the computing
+    // warps have stored by then.
+    if (__any_sync(kFull, above != 0u) && lane == 0) s.above = 1;
+    __syncwarp();
+    if (lane == 0) BarrierArrive(SharedAddress(&s.seen));
+    bool all = BarrierWait(SharedAddress(&s.seen), 0, &s.failed);
+    if (!__all_sync(kFull, all) || s.above == 0) return;
+    all = BarrierWait(SharedAddress(&s.stored), 0, &s.failed);
+    if (!__all_sync(kFull, all)) return;
+    for (int index = blockIdx.x; index < tasks; index += gridDim.x) {
+      const MvTask task = task_at(index);
+      for (int64_t p0 = task.begin; p0 < task.end; p0 += 8) MvAgain<T, kGroup, kRows>(a, task, p0, lt >> 5);
     }
     return;
   }
@@ -451,6 +527,8 @@ __global__ void __launch_bounds__(kMvThreads + 32 + kMvLayout, 2)
       }
     }
   }
+  __syncwarp();
+  if (lane == 0) BarrierArrive(SharedAddress(&s.stored));
 }
 
 template <typename T, int kGroup, int kParts>

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from tensor0_b200 import _native, build, routed
-from test_routed import A, B, C, D, E, F, G, H, HALF, TYPES, call, make_routing, near, plain_choice, wide
+from test_routed import (A, B, C, D, E, F, G, H, HALF, TYPES, call, make_routing, near, plain_choice, plain_product,
+                         wide)
 
 gpu = pytest.mark.gpu
 
@@ -104,6 +105,65 @@ def test_gates_far_below_zero_keep_bf16_range():
     both = np.concatenate([u * (s + g * s * (1 - s)), g * s])
     size = np.concatenate([np.abs(u) * (s + np.abs(g * s)), np.abs(g * s)])
     near(h_grad[0], both, 1.01 * 2.0 ** -8 * np.abs(both) + slack * size + 2.0 ** -134 + 200 * 2.0 ** -149, "gradient")
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# 4-bit products
+
+
+def plain_four(codes, scales, group):
+    q = np.stack([codes.numpy() & 15, codes.numpy() >> 4], 3).reshape(codes.shape[0], codes.shape[1], -1)
+    return (q.astype(np.float64) - 8) * np.repeat(wide(scales), group, axis=2)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("tokens, experts, top_k, inner, outer, group",
+                         [(1, 4, 2, 64, 24, 32), (5, 3, 2, 1152, 40, 64), (20, 2, 2, 2176, 300, 128),
+                          (3, 7, 2, 96, 33, 32)])
+def test_infinite_rows_through_4_bit_weights(tokens, experts, top_k, inner, outer, group, dtype):
+    """An infinity times a weight is an infinity of the product's sign (NaN times a weight of zero, and NaN where
+    infinities of both signs meet), in its own row only."""
+    kind, unit, tiny = HALF[dtype]
+    host, r = make_routing(tokens, experts, top_k, 31)
+    g = torch.Generator().manual_seed(inner)
+    x = torch.randn(tokens, inner, generator=g).to(kind)
+    x[0, inner - 3] = math.inf
+    if tokens > 2:
+        x[1, 7], x[2, 1], x[2, inner // 2] = -math.inf, math.inf, math.nan
+    if tokens > 4:
+        x[4, 5], x[4, inner - 1] = math.inf, math.inf
+    codes = torch.randint(0, 256, (experts, outer, inner // 2), generator=g, dtype=torch.uint8)
+    codes[:, 0] = 0x88                                    # a row of zero weights
+    scales = ((0.1 + torch.rand(experts, outer, inner // group, generator=g)) / math.sqrt(inner)).to(kind)
+    got = routed.routed_matvec(x.cuda(), routed.Int4Weights(codes.cuda(), scales.cuda(), group), r, gather=True)
+    w = plain_four(codes, scales, group)
+    with np.errstate(all="ignore"):
+        y, size = plain_product(host, wide(x), w.transpose(0, 2, 1), True, top_k)
+        spread = np.broadcast_to(np.repeat(wide(scales), group, axis=2), w.shape)
+        excess, _ = plain_product(host, np.abs(wide(x)), spread.transpose(0, 2, 1), True, top_k)
+    assert np.isinf(y).any() and np.isnan(y).any()
+    # A group's sum is one of (16 + q) x from -24 x on, whatever its weights are; the groups' sums are added.
+    error = group * 2.0 ** -23 * 55 * excess + inner // group * 2.0 ** -23 * size
+    near(got, y, np.where(np.isfinite(y), 1.01 * unit * np.abs(y) + tiny + error, 0.0), "rows")
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_large_rows_through_4_bit_weights(group):
+    """BF16 values whose products fit 32 bits, though 16 times them, or their sum, would not."""
+    inner, outer = 256, 40
+    host, r = make_routing(4, 2, 1, 32)
+    g = torch.Generator().manual_seed(group)
+    x = torch.randn(4, inner, generator=g).bfloat16()
+    x[0, 3], x[0, 9] = 2e37, 2e37
+    x[1, 3], x[1, 200] = 2e37, -2e37
+    x[2] = 1e36
+    codes = torch.randint(0, 256, (2, outer, inner // 2), generator=g, dtype=torch.uint8)
+    scales = torch.full((2, outer, inner // group), 2.0 ** -6).bfloat16()
+    got = routed.routed_matvec(x.cuda(), routed.Int4Weights(codes.cuda(), scales.cuda(), group), r, gather=True)
+    y, size = plain_product(host, wide(x), plain_four(codes, scales, group).transpose(0, 2, 1), True, 1)
+    near(got, y, 1.01 * 2.0 ** -8 * np.abs(y) + inner * 2.0 ** -23 * size, "rows")
 
 
 # ----------------------------------------------------------------------------------------------------------------
