@@ -154,9 +154,9 @@ __global__ void __launch_bounds__(kTcThreads + (kGather ? kGatherThreads : 0), 1
     s.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (tid == 32) {
-    PrefetchMap(&a.a);
-    PrefetchMap(&a.b);
+  if (tid == 32) {   // a gathered operand has no map
+    if (!kGather || a.gather_a == 0) PrefetchMap(&a.a);
+    if (!kGather || a.gather_b == 0) PrefetchMap(&a.b);
   }
   WaitForPrevious();
   for (int e = tid; e <= a.experts; e += blockDim.x) {
