@@ -3,7 +3,9 @@ than one thread.  Tolerances are those of ``test_routed``: they follow from the 
 
 import math
 import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -12,6 +14,9 @@ import torch
 from tensor0_b200 import _native, build, routed
 from test_routed import (A, B, C, D, E, F, G, H, HALF, TYPES, call, make_routing, near, plain_choice, plain_product,
                          wide)
+
+sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "examples"))
+import routed_layer  # noqa: E402
 
 gpu = pytest.mark.gpu
 
@@ -69,7 +74,7 @@ def test_a_choice_by_scores_surfaces_numbers_that_are_not(experts, groups, top_g
 def test_checkpoint_of_an_infinity_is_not_a_number(value, width, group, dtype):
     """The whole group of an infinite value loads as NaN, and its gradient is NaN: no infinity of the other sign."""
     h = torch.randn(3, 2 * width, generator=torch.Generator().manual_seed(width)).to(HALF[dtype][0])
-    gate, up = 5, width + width - 1                       # one in the first group of the gate, one in the last of the up
+    gate, up = 5, width + width - 1                       # the gate's first group, the up's last
     h[1, gate] = h[2, up] = value
     _, kept = routed.gated_save(h.cuda(), group=group)
     column = np.arange(2 * width)
@@ -164,6 +169,82 @@ def test_large_rows_through_4_bit_weights(group):
     got = routed.routed_matvec(x.cuda(), routed.Int4Weights(codes.cuda(), scales.cuda(), group), r, gather=True)
     y, size = plain_product(host, wide(x), plain_four(codes, scales, group).transpose(0, 2, 1), True, 1)
     near(got, y, 1.01 * 2.0 ** -8 * np.abs(y) + inner * 2.0 ** -23 * size, "rows")
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# Strides and graphs
+
+
+@gpu
+@pytest.mark.parametrize("begin", [0, 3, 8])
+def test_rows_of_wider_tensors(begin):
+    """Every row operand as columns of a wider tensor, on 16-byte boundaries and off them: the bits of a copy."""
+    host, r = make_routing(60, 6, 3, 41)
+    g = torch.Generator().manual_seed(begin)
+    store = torch.randn(180, 320, generator=g).half().cuda()
+    wider = torch.randn(60, 320, generator=g).half().cuda()
+
+    def part(rows, width):
+        return rows[:, begin:begin + width]
+    y = part(store, 136)
+    assert torch.equal(routed.routed_sum(y, r), routed.routed_sum(y.contiguous(), r))
+    h = part(store, 272)
+    a, kept = routed.gated_save(h, routing=r)
+    copied, copied_kept = routed.gated_save(h.contiguous(), routing=r)
+    assert all(torch.equal(one, other) for one, other in zip((a, *kept[:2]), (copied, *copied_kept[:2])))
+    assert torch.equal(routed.gated(h, routing=r), a)
+    da = part(store, 136)
+    strided = routed.gated_backward(kept, da, routing=r)
+    for one, other in zip(strided, routed.gated_backward(kept, da.contiguous(), routing=r)):
+        # Off the boundaries a lane has other columns: the weight's gradient is summed in another order.
+        if one.dtype == torch.float16:
+            assert torch.equal(one, other)
+        else:
+            assert torch.allclose(one, other, rtol=0, atol=136 * 2.0 ** -23 * 60)
+    x = part(wider, 64)
+    for gather_y in (False, True):
+        dy = part(wider if gather_y else store, 136)
+        got = routed.routed_weight_grad(x, dy, r, gather_x=True, gather_y=gather_y)
+        expected, size = np.zeros((6, 64, 136)), np.zeros((6, 64, 136))
+        for e in range(6):
+            p = np.arange(host[4][e], host[4][e + 1])
+            left, right = wide(x)[host[2][p] // 3], wide(dy)[host[2][p] // 3 if gather_y else p]
+            expected[e], size[e] = left.T @ right, np.abs(left).T @ np.abs(right)
+        near(got, expected, 1.01 * 2.0 ** -11 * np.abs(expected) + 2.0 ** -25 + 180 * 2.0 ** -23 * size)
+    codes = torch.randint(0, 256, (6, 40, 32), generator=g, dtype=torch.uint8).cuda()
+    four = routed.Int4Weights(codes, torch.rand(6, 40, 2, generator=g).half().cuda(), 32)
+    assert torch.equal(routed.routed_matvec(x, four, r, gather=True),
+                       routed.routed_matvec(x.contiguous(), four, r, gather=True))
+    rows = part(store, 64)
+    assert torch.equal(routed.routed_matvec(rows, four, r), routed.routed_matvec(rows.contiguous(), four, r))
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_a_captured_layer_repeats_its_results(tokens):
+    layer = routed_layer.RoutedLayer(128, 64, 8, 2, seed=7)
+    served = routed_layer.ServedLayer(layer)
+    x = torch.randn(tokens, 128, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    y_grad = torch.randn(tokens, 128, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+
+    def step():
+        y, saved = layer.forward(x)
+        x_grad, grads = layer.backward(saved, y_grad)
+        return (y, x_grad, *grads, served(x))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (3, 4):
+        x.copy_(torch.randn(tokens, 128, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        for one, other in zip(captured, step()):
+            assert torch.equal(one, other)
 
 
 # ----------------------------------------------------------------------------------------------------------------
@@ -264,7 +345,8 @@ class Product(torch.autograd.Function):
         x, w, *routing = ctx.saved_tensors
         r = routed.Routing(*routing)
         rows = routed.routed_matmul(y_grad, w, r, gather=True, transpose=True)
-        return routed.routed_sum(rows, r), routed.routed_weight_grad(x, y_grad, r, gather_x=True, gather_y=True), *[None] * 5
+        w_grad = routed.routed_weight_grad(x, y_grad, r, gather_x=True, gather_y=True)
+        return routed.routed_sum(rows, r), w_grad, *[None] * 5
 
 
 @gpu
@@ -346,8 +428,8 @@ int main() {
 def test_a_kernels_shared_memory_limit_only_grows(tmp_path):
     source, program = tmp_path / "limit.cu", tmp_path / "limit"
     source.write_text(SHARED_LIMIT)
-    subprocess.run([build.nvcc(), *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr", "-I", str(build.CSRC), str(source),
-                    "-o", str(program)], check=True)
+    subprocess.run([build.nvcc(), *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr", "-I", str(build.CSRC),
+                    str(source), "-o", str(program)], check=True)
     assert subprocess.run([str(program)], timeout=60).returncode == 0
 
 
@@ -386,7 +468,8 @@ def test_gated_results_over_the_routings_offsets_are_refused(name, arguments):
     assert status == 1 and "overlap" in text, text
 
 
-@pytest.mark.parametrize("tokens, experts", [(1000, 513), (1000, 1 << 30), (MOST + 1, 8), (1 << 60, 8), (-1, 8), (1000, 0)])
+@pytest.mark.parametrize("tokens, experts", [(1000, 513), (1000, 1 << 30), (MOST + 1, 8), (1 << 60, 8), (-1, 8),
+                                             (1000, 0)])
 def test_a_route_that_is_refused_needs_no_workspace(tokens, experts):
     """The binding asks for the size before the router checks its arguments: no memory for what it refuses."""
     build.build()
