@@ -586,9 +586,10 @@ __global__ void __launch_bounds__(kPlaceThreads) RoutePlace(RouteArgs a, int64_t
 //   renormalised: g <- (g - sum(g p) / total) / total, total = sum p + 1e-20
 //   softmax: dx_j = s_j (ds_j - sum(g p)),  ds the scattered g
 //   sigmoid: dx_j = ds_j s_j (1 - s_j)
-// Reads and writes each logit once; the scores are recomputed, with the fast
-// exponential (about 1e-6 of a score far below the largest, less near it).  A
-// warp has one token: instructions bound it, and a loop's cost more than launching.
+// Reads and writes each logit once; the scores are recomputed.  (The fast
+// exponential is off by 4e-6 of a score 80 below the largest, which a bias or a
+// group may have chosen.)  A warp has one token: instructions bound it, and a
+// loop's cost more than launching.
 template <typename T, int V, bool kSoftmax>
 __global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs a, bool vector) {
   __shared__ __align__(16) float scattered[kRouteThreads / 32][32 * V];   // ds
@@ -618,15 +619,15 @@ __global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        x[j] = __expf(x[j] - top);
+        x[j] = expf(x[j] - top);
         sum += x[j];
       }
       const float inverse = __fdividef(1.0f, WarpSum(sum));
-      p = __expf(logit - top) * inverse;
+      p = expf(logit - top) * inverse;
 #pragma unroll
       for (int j = 0; j < V; ++j) x[j] *= inverse;
     } else {
-      p = __fdividef(1.0f, 1.0f + __expf(-logit));
+      p = __fdividef(1.0f, 1.0f + expf(-logit));
     }
     if (a.renormalize != 0) {
       // The weight is rounded as in the forward pass: a single choice's is 1 and

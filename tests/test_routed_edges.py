@@ -63,6 +63,42 @@ def test_a_choice_by_scores_surfaces_numbers_that_are_not(experts, groups, top_g
     assert torch.isnan(grad[:4]).any(1).all() and (grad[4] == 0).all() and torch.isfinite(grad[5:]).all()
 
 
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_gradient_of_choices_far_below_the_largest(renormalize, score):
+    """A bias picks experts whose scores are small: their gradient is as exact as any other's."""
+    g = torch.Generator().manual_seed(5)
+    logits = -torch.randint(8 * 20, 8 * 70, (100, 32), generator=g).float() / 8      # differences are exact
+    logits[:, 0] = 0.0
+    bias = torch.zeros(32)
+    bias[1:4] = 8.0
+    r = routed.route(logits.cuda(), 3, score=score, renormalize=renormalize, bias=bias.cuda())
+    assert (r.experts.sort(1).values.cpu() == torch.tensor([1, 2, 3])).all()
+    up = torch.randn(100, 3, generator=g).cuda()
+    got = wide(routed.route_backward(logits.cuda(), r, up, score=score, renormalize=renormalize))
+    x, chosen, grad = wide(logits), r.experts.long().cpu().numpy(), wide(up)
+    e = np.exp(x)
+    s = e / e.sum(1, keepdims=True) if score == "softmax" else 1 / (1 + np.exp(-x))
+    p = np.take_along_axis(s, chosen, 1)
+    size = np.abs(grad)
+    if renormalize:
+        total = p.sum(1, keepdims=True) + 1e-20
+        mean = (grad * p / total).sum(1, keepdims=True)
+        size = (size + (size * p / total).sum(1, keepdims=True)) / total
+        grad = (grad - mean) / total
+    ds, ds_size = np.zeros_like(s), np.zeros_like(s)
+    np.put_along_axis(ds, chosen, grad, 1)
+    np.put_along_axis(ds_size, chosen, size, 1)
+    if score == "softmax":
+        expected = s * (ds - (grad * p).sum(1, keepdims=True))
+        magnitude = s * (ds_size + (size * p).sum(1, keepdims=True))
+    else:
+        expected, magnitude = ds * s * (1 - s), ds_size * s
+    # Two exponentials of 2 units of 2^-23, their sums, three divisions of 2 and about five roundings: 16 units.
+    near(torch.from_numpy(got), expected, 16 * 2.0 ** -23 * magnitude + 1e-37, "logits")
+
+
 # ----------------------------------------------------------------------------------------------------------------
 # Gated activation and its checkpoint
 
