@@ -191,7 +191,7 @@ def checkpoint_load(checkpoint: Checkpoint, dtype: torch.dtype = torch.float32) 
 @torch.no_grad()
 def pack_int4(w: torch.Tensor, group: int = 128) -> Int4Weights:
     """``w`` [experts, inner, outer] in 4 bits: per group of ``group`` inner neighbours the scale max|w| / 7 (in w's
-    type) and whole numbers from -7 to 7.  Done once per model, in plain torch."""
+    type) and whole numbers from -7 to 7.  A NaN or infinity makes its group NaN.  Done once per model, in plain torch."""
     if w.dim() != 3 or w.dtype not in _HALF:
         raise ValueError("weights must be [experts, inner, outer] of float16 or bfloat16")
     if group not in (32, 64, 128) or w.shape[1] % group:
@@ -199,8 +199,10 @@ def pack_int4(w: torch.Tensor, group: int = 128) -> Int4Weights:
     experts, inner, outer = w.shape
     by_group = w.transpose(1, 2).float().reshape(experts, outer, inner // group, group)
     scales = (by_group.abs().amax(3) / 7).to(w.dtype)
-    unit = torch.where(scales == 0, 1, scales).float()
-    codes = (torch.round(by_group / unit[..., None]).clamp(-7, 7) + 8).to(torch.uint8).reshape(experts, outer, inner)
+    fine = torch.isfinite(scales)
+    unit = torch.where(fine & (scales != 0), scales, 1).float()
+    scales = torch.where(fine, scales, torch.nan)
+    codes = (torch.round(by_group / unit[..., None]).nan_to_num().clamp(-7, 7) + 8).to(torch.uint8).reshape(experts, outer, inner)
     return Int4Weights((codes[..., 0::2] | (codes[..., 1::2] << 4)).contiguous(), scales.contiguous(), group)
 
 

@@ -207,6 +207,19 @@ def test_large_rows_through_4_bit_weights(group):
     near(got, y, 1.01 * 2.0 ** -8 * np.abs(y) + inner * 2.0 ** -23 * size, "rows")
 
 
+@gpu
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_packed_weights_that_are_not_finite_stay_so(value):
+    """A weight that has no 4-bit code makes its group NaN, and no infinity of the other sign or finite value."""
+    w = torch.randn(2, 128, 6, generator=torch.Generator().manual_seed(3)).bfloat16()
+    w[1, 40, 2] = value
+    _, r = make_routing(8, 2, 2, 33)
+    got = routed.routed_matvec(torch.ones(8, 128).bfloat16().cuda(), routed.pack_int4(w.cuda(), 32), r, gather=True)
+    bad = torch.zeros(16, 6, dtype=torch.bool)
+    bad[int(r.offsets[1]):, 2] = True                     # expert 1's rows
+    assert torch.equal(torch.isnan(got).cpu(), bad) and torch.isfinite(got.cpu()[~bad]).all()
+
+
 # ----------------------------------------------------------------------------------------------------------------
 # Strides and graphs
 
