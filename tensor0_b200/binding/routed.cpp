@@ -3,9 +3,10 @@
 //
 // A serving step calls these for one token, where the operators take 4 to 8 us:
 // the argument checks and the call are compiled (4 to 6 us a call with its
-// launch and result; the same checks in Python and ctypes took 11 to 14).  Shapes, types, strides and
-// devices are checked here, values, sizes and overlaps by the entry points.
-// Every refusal is a ValueError, every other failure a RuntimeError.
+// launch and result; the same checks in Python and ctypes took 11 to 14).  Shapes,
+// types, strides, devices and autograd are checked here, values, sizes and overlaps
+// by the entry points.  Every refusal is a ValueError, every other failure a
+// RuntimeError.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>

@@ -11,10 +11,11 @@
 // w is the row's routing weight (1 without a routing); rows that belong to no
 // expert are not read, and zeros are written for them.
 //
-// Measured: saving 12294 rows of 1416 (f16, groups of 64) 33 us, 141 MB, and
-// loading them 18 us, 106 MB: bound by instructions as much as by memory.  The
-// gradient of 65536 rows of 2048 (bf16) 224 us, 1.35 GB, 0.92 of the copy
-// bandwidth.  Widths that 8 does not divide take 1.3 to 1.6 times as long.
+// Measured, replayed with three inputs by turns: saving 12294 rows of 1416 (f16,
+// groups of 64) 35 us, 141 MB, and loading them 21 us, 106 MB: bound by instructions
+// as much as by memory.  The gradient of 65536 rows of 2048 (bf16) 225 us, 1.35 GB,
+// 0.91 of the copy bandwidth; the activation alone 144 us, 0.81 GB, 0.85.  Widths that
+// 8 does not divide take 1.2 to 1.7 times as long.
 #include <algorithm>
 #include <type_traits>
 

@@ -12,7 +12,7 @@
 // Both are exact.  What is added to each weight (8 too much, or 24) is taken
 // off by starting a group's 32-bit sum at minus that times the sum of x, and
 // the scale multiplies the group's sum, so nothing is rounded before the result.
-// Values that these sums do not hold, infinities or BF16 ones from 2^115 on, are
+// Values that these sums do not hold, infinities or BF16 ones from 2^115 (4e34) on, are
 // rare: eight token rows with one among them are computed again, by the formula as
 // it stands (MvAgain; 16 tokens to 4 of 64 experts at 4096 x 2048 with an infinity
 // each 1.4 ms).  Looking for them costs 0.2 us of a small call, 1 % of a large one.
@@ -26,9 +26,10 @@
 // touch eight rows per instruction: the load path was the bound at twice the
 // time.)  An expert's weights are read once for every eight of its rows.
 //
-// Measured: one token to 8 of 64 experts at 2048 x 1024 6.4 us; 16 tokens to 4
-// of 64 at 4096 x 2048 43 us, 180 MB (4.2 TB/s): 656 tasks on 296 blocks are
-// three rounds for 2.2, and the computing warps issue in two of three cycles.
+// Measured, replayed with three inputs by turns: one token to 8 of 64 experts at
+// 2048 x 1024 6.7 us; 16 tokens to 4 of 64 at 4096 x 2048 44 us, 180 MB (4.1 TB/s):
+// 656 tasks on 296 blocks are three rounds for 2.2, and the computing warps issue in
+// two of three cycles.
 #include <algorithm>
 
 #include "engine.h"
@@ -554,7 +555,15 @@ void Launch(const MatvecArgs& a, cudaStream_t stream) {
 template <typename T, int kGroup>
 void ByParts(const MatvecArgs& a, cudaStream_t stream) {
   // Fewer parts read longer runs of the deep axis per warp; more parts give
-  // more blocks.
+  // more blocks.  Replayed, with 1, 2 and 4 parts, tokens to top_k of experts:
+  //    1 to 8 of  64, 2048 x 1024:  10.2   8.7   6.5 us (4 taken)
+  //    4 to 8 of  64, 2048 x 1024:  15.1  14.9  16.7    (4)
+  //    8 to 4 of  32, 4096 x 2048:  37.2  38.3  42.3    (2)
+  //    8 to 8 of 128, 2048 x 1024:  25.1  25.8  28.1    (2)
+  //   16 to 4 of  64, 4096 x 2048:  43.4  47.5  61.3    (1)
+  //   16 to 8 of 128, 2048 x 1024:  33.0  35.0  42.8    (1)
+  // It goes by blocks and not by the rounds they make: 64 tokens to 1 of 16 at
+  // 4096 x 1500 take 36.3 us with 2 parts and 47.5 with the 4 taken.
   const int64_t blocks = std::min<int64_t>(a.experts, a.entries) * ((a.outer + 127) / 128);
   const int resident = RoutedSmCount() * 2;
   if (blocks >= 2 * resident) Launch<T, kGroup, 1>(a, stream);

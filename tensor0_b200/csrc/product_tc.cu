@@ -23,12 +23,13 @@
 // memory, in both operands, so that a value that is not finite stays with its
 // own expert.
 //
-// Measured, bf16: 32768 rows of 64 experts, 1024 x 2048, 133 us (1.0 PFLOP/s,
-// 0.64 of the matrix rate; every second expert's last tile is half empty); of 32
-// experts at 2048 x 2048 220 us (1.25); that weight gradient 250 us, with gathered
-// rows 275 (x) or 303 (y).  9222 rows of 40 experts at 1000 x 1416 f16 48 us, where reading the
-// weights takes 17.  What bounds: the slices' latency against four stages, and at
-// few rows per expert the weights' bytes.
+// Measured, bf16, replayed with three inputs by turns: 32768 rows of 64 experts,
+// 1024 x 2048, 136 us (1.0 PFLOP/s, 0.61 of the matrix rate; every second expert's
+// last tile is half empty); of 32 experts at 2048 x 2048 223 us (1.23 PFLOP/s),
+// transposed 248; that weight gradient 245 us, with gathered rows 272 (x) or 309 (y).
+// 9222 rows of 40 experts at 1000 x 1416 57 us, where reading the weights takes 17.
+// What bounds: the slices' latency against four stages, and at few rows per expert
+// the weights' bytes.
 // Slower: two blocks sharing 256 x 256 tiles (cta_group::2), 265 us where this
 // took 232, for the tiles' empty halves and the blocks' handshakes; eight storing
 // warps, 34 us instead of 30 for the weight gradient of 64 rows of 32 experts,

@@ -21,9 +21,10 @@
 // counts summed over the blocks before each, entries placed.  Few tokens take
 // one block that does it all.
 //
-// Measured: 8 tokens of 64 experts 3.8 us; 8191 of 256 in groups with a bias
-// 24 us (choice 17); 32768 of 128 forward and backward 41 us (choice 24,
-// gradient 11, where reading and writing the logits takes 6).
+// Measured, replayed with three inputs by turns: 8 tokens of 64 experts 4.0 us; 8191
+// of 256 in groups with a bias 24 us (choice 17); 32768 of 128 forward and backward
+// 42 to 44 us (choice 24, gradient 11, where reading and writing the logits takes
+// 6).  As calls one after the other: 4.2, 27 and 50 us.
 #include <algorithm>
 #include <climits>
 
@@ -654,7 +655,10 @@ __global__ void __launch_bounds__(kRouteThreads) RouteBackward(RouteBackwardArgs
   StoreValues<T, V>(static_cast<T*>(a.logits_grad) + int64_t{t} * a.experts, a.experts, lane, vector, d);
 }
 
-// Up to this many tokens one block does the whole call.
+// Up to this many tokens one block does the whole call.  Replayed, one block and
+// three launches, 64 experts: 8 tokens 3.9 and 7.6 us, 64 7.1 and 7.9, 96 8.8 and 8.0;
+// 16 experts: 64 tokens 5.7 and 7.3, 128 8.3 and 7.5.  (With 256 experts and a bias the
+// launches are ahead from 48 tokens on, 11.3 us for 14.2.)
 constexpr int64_t kOneBlockTokens = 64;
 
 // Counting blocks: enough to fill the device with warps, each with its eight
@@ -678,8 +682,9 @@ void Route(const RouteArgs& a, cudaStream_t stream) {
   const int64_t per_block = TokensPerBlock(a.tokens);
   const unsigned blocks = static_cast<unsigned>((a.tokens + per_block - 1) / per_block);
   const std::size_t select = (bins + (a.groups > 1 ? kRouteThreads / 32 * bins : 0)) * sizeof(int);
-  // While the choice is short, the two launches after it are worth hiding (8191
-  // tokens: 27 us instead of 31; 32768: 56 instead of 54).
+  // While the choice is short, the two launches after it are worth hiding (calls one
+  // after the other, 8191 tokens: 27 us instead of 31; 32768, with the gradient: 53
+  // instead of 50).
   const bool close = per_block <= 16;
   LaunchRouted("router launch", BriefGrid(blocks), RouteSelect<T, V, kByLogit>, blocks, kRouteThreads, select, stream, a, per_block, vector);
   LaunchRouted("row order launch", close, RouteScan, static_cast<unsigned>((a.experts + kScanExperts - 1) / kScanExperts),

@@ -101,9 +101,10 @@ __device__ __forceinline__ void LetNextStart() { asm volatile("griddepcontrol.la
 __device__ __forceinline__ void WaitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Launches a kernel that begins with these two.  brief: it may start while the
-// kernel before it runs.  That takes 0.3 to 0.8 us off calls of 4 to 8 us (a
-// route of 8 tokens, a product of 64), and costs long ones a few percent (the
-// product and sum of 8192 tokens 172 us instead of 166), so those do without.
+// kernel before it runs.  That takes 2 us off calls of 4 to 8 us that follow one
+// another (a route of 8 tokens 4.2 us instead of 6.1, a product of 64 6.3 instead of
+// 8.2), and costs long ones a few percent (the product and sum of 8192 tokens 196 us
+// instead of 189), so those do without.
 template <typename... Parameters, typename... Arguments>
 void LaunchRouted(const char* what, bool brief, void (*kernel)(Parameters...), dim3 blocks, unsigned threads, std::size_t smem,
                   cudaStream_t stream, Arguments&&... arguments) {
