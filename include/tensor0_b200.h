@@ -294,12 +294,13 @@ int t0b_sector_gemm(int32_t dtype, int64_t sectors, const int64_t* host_table,
  * their best c (group_best 1) or the sum of their two best (2); then the top_k
  * best c, ties to the lowest index.  weights = scale * s, divided by the sum of
  * the chosen s + 1e-20 if renormalize is 1.  A logit of -inf or NaN takes no
- * expert; a token with mask 0 takes none and its logits are not read.  Under
- * softmax a NaN or +inf logit makes the token's weights NaN; its choice goes by
- * the scores without the NaN logits, and by their limits at +inf.  Missing
- * choices have index -1, weight 0 and position -1.  experts <= 512, top_k <= 32,
- * groups <= 32.  workspace: t0b_route_workspace() bytes for the current device,
- * 4-byte aligned (may be NULL when that is 0, as it is for refused sizes).
+ * expert, and an expert whose bias is either is not chosen; a token with mask 0
+ * takes none and its logits are not read.  Under softmax a NaN or +inf logit makes
+ * the token's weights NaN; its choice goes by the scores without the NaN logits,
+ * and by their limits at +inf.  Missing choices have index -1, weight 0 and
+ * position -1.  experts <= 512, top_k <= 32, groups <= 32.  workspace:
+ * t0b_route_workspace() bytes for the current device, 4-byte aligned (may be NULL
+ * when that is 0, as it is for refused sizes).
  */
 size_t t0b_route_workspace(int64_t tokens, int32_t experts);
 int t0b_route(int32_t dtype, int64_t tokens, int32_t experts, int32_t top_k, int32_t groups, int32_t top_groups,

@@ -106,8 +106,9 @@ def route(logits: torch.Tensor, top_k: int, *, groups: int = 1, top_groups: int 
     (``group_best`` 1) or sum of the two best (2) stay.  ``renormalize`` divides the chosen scores by their sum.
     ``mask`` (bool [tokens]): tokens that are False take no expert, whatever their logits hold.
 
-    A logit of -inf or NaN takes no expert.  Under softmax a NaN or +inf logit makes its token's weights NaN; the choice
-    then goes by the scores without the NaN logits, and by their limits at +inf.
+    A logit of -inf or NaN takes no expert, and an expert whose bias is either is not chosen.  Under softmax a NaN or
+    +inf logit makes its token's weights NaN; the choice then goes by the scores without the NaN logits, and by their
+    limits at +inf.
     """
     if out is None:
         if logits.dim() != 2:

@@ -65,6 +65,23 @@ def test_a_choice_by_scores_surfaces_numbers_that_are_not(experts, groups, top_g
 
 @gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("best", [1, 2])
+def test_a_bias_excludes_experts(best, score):
+    """An expert whose bias is -inf or NaN is not chosen; the others are as if its score were out of the choice."""
+    g = torch.Generator().manual_seed(8)
+    logits, bias = torch.randn(90, 32, generator=g), 0.3 * torch.randn(32, generator=g)
+    bias[3], bias[17] = math.nan, -math.inf
+    plain = {"groups": 4, "top_groups": 2, "group_best": best, "score": score}
+    r = routed.route(logits.cuda(), 4, bias=bias.cuda(), **plain)
+    low = bias.clone()
+    low[[3, 17]] = -1e30                                  # below every other
+    expected = routed.route(logits.cuda(), 4, bias=low.cuda(), **plain)
+    assert not torch.isin(r.experts.cpu(), torch.tensor([3, 17])).any() and torch.isfinite(r.weights).all()
+    assert all(torch.equal(a, b) for a, b in zip(r, expected))
+
+
+@gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])
 def test_gradient_of_choices_far_below_the_largest(renormalize, score):
     """A bias picks experts whose scores are small: their gradient is as exact as any other's."""
