@@ -23,8 +23,8 @@
 //
 // Measured, replayed with three inputs by turns: 8 tokens of 64 experts 4.0 us; 8191
 // of 256 in groups with a bias 24 us (choice 17); 32768 of 128 forward and backward
-// 42 to 44 us (choice 24, gradient 11, where reading and writing the logits takes
-// 6).  As calls one after the other: 4.2, 27 and 50 us.
+// 42 to 44 us (choice 24, gradient 11 or, with cold caches, 14, where reading and
+// writing the logits takes 6).  As calls one after the other: 4.2, 27 and 50 us.
 #include <algorithm>
 #include <climits>
 
